@@ -85,6 +85,12 @@ class ArgmaxResult(C.Structure):
                 ("status", C.c_int32), ("reserved", C.c_int32)]
 
 
+class Kv4Pool(C.Structure):
+    """A pool of 4-bit KV pages on the device (pages_dev: address of page 0)."""
+    _fields_ = [("pages_dev", C.c_void_p), ("page_count", C.c_uint32), ("num_layers", C.c_uint32),
+                ("num_kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
 class EligibleGreedyResult(C.Structure):
     """glacier_hip_eligible_greedy_result_t (EligibleGreedyResult,
     int4_executor.zig:786-801, plus the rows this device streamed)."""
@@ -622,6 +628,23 @@ _SIGS = [
     ("glacier_hip_paged_attention_prefill", C.c_int,
      [_P, _P, _P, _P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
       C.c_uint32, C.c_uint32, _P, _P]),
+    ("glacier_hip_kv4_page_bytes", C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    ("glacier_hip_kv_plan_rows", C.c_int,
+     [_P, _P, _P, C.c_uint32, C.c_uint32, _P, C.c_uint32, _P, C.c_uint32, _P, _P, _P, _P, _P, _P, _P,
+      _P]),
+    ("glacier_hip_kv4_append", C.c_int,
+     [_P, C.POINTER(Kv4Pool), C.c_uint32, _P, _P, C.c_int, C.c_uint64, C.c_uint64, _P, C.c_uint32,
+      _P]),
+    ("glacier_hip_kv4_read", C.c_int,
+     [_P, C.POINTER(Kv4Pool), C.c_uint32, _P, C.c_uint32, _P, _P, _P]),
+    ("glacier_hip_kv4_attention_workspace_bytes", C.c_uint64,
+     [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]),
+    ("glacier_hip_paged_attention_kv4", C.c_int,
+     [_P, C.POINTER(Kv4Pool), C.c_uint32, _P, _P, C.c_uint32, _P, C.c_uint32, C.c_uint32, C.c_uint32,
+      _P, _P, C.c_uint64, _P]),
+    ("glacier_hip_paged_attention_kv4_rows", C.c_int,
+     [_P, C.POINTER(Kv4Pool), C.c_uint32, _P, _P, C.c_uint32, _P, _P, C.c_uint32, C.c_uint32,
+      C.c_uint32, C.c_uint32, _P, _P, C.c_uint64, _P]),
     ("glacier_hip_argmax", C.c_int, [_P, _P, C.c_uint64, C.c_uint32, _P, _P]),
     ("glacier_hip_eligible_argmax", C.c_int,
      [_P, _P, C.c_uint64, _P, C.c_uint64, C.c_uint32, C.POINTER(ArgmaxResult), _P]),

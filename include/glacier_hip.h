@@ -394,6 +394,130 @@ int glacier_hip_paged_attention_o(glacier_hip_context *ctx, const float *q_dev,
                                   const glacier_hip_int4_weight *o_weight, float *parts_dev,
                                   void *stream);
 
+/* ---- 4-bit paged KV: planning, storing and attending -----------------------
+ * No counterpart in the reference, whose pages are f32. Pages of 16 positions
+ * hold K and V of every layer as 4-bit codes with fp16 steps and minima per
+ * position and group of 32 dims of a KV head: 5 bits an element. A stored
+ * value is
+ *     code * step + minimum,   code = 0..15,
+ * where, for the group's f32 values x, minimum = fp16(min x), step =
+ * fp16((max x - min x) / 15) (difference and quotient rounded to f32), code =
+ * (x - minimum) / step rounded once to the nearest integer, ties to even, and
+ * clamped to 0..15 (0 where step is 0). A group holding a NaN, an infinity or
+ * a magnitude above 32768 is stored as NaN.
+ *
+ * page[layer][KV head][K, V][10 * head_dim bytes]; in a tile, for position P
+ * (0..15), NG = head_dim / 32 and NH = head_dim / 64,
+ *   K codes  byte P * head_dim / 2 + (c * NG + g) * 4 + b: dims 32 g + 8 c +
+ *            2 b (low nibble) and the next of position P,
+ *   V codes  byte ((((P / 4) * 16 + j) * 2 + P / 2 % 2) * NH + h) * 4 +
+ *            P % 2 * 2 + b: dims 16 (4 h + 2 b) + j (low nibble) and
+ *            16 (4 h + 2 b + 1) + j of position P,
+ *   from byte 8 * head_dim  steps  [P / 4][g][P % 4] of K and of V,
+ *   from byte 9 * head_dim  minima [P][g] of K, [P / 4][g][P % 4] of V
+ * (the order the attention kernels' matrix operands take them in).
+ * head_dim is 64 or 128, pages_dev aligned to 16 bytes. */
+typedef struct {
+    void *pages_dev;             /* [page_count][glacier_hip_kv4_page_bytes] */
+    uint32_t page_count;
+    uint32_t num_layers;
+    uint32_t num_kv_heads;
+    uint32_t head_dim;
+} glacier_hip_kv4_pool_t;
+
+#define GLACIER_HIP_KV_MAX_LANES 1024u     /* lanes of a plan or an attention call */
+#define GLACIER_HIP_KV_MAX_ROWS 1048576u   /* rows of a plan, an append, a read, an attention call */
+
+/* Bytes of one page, 20 * num_layers * num_kv_heads * head_dim (0: a head_dim
+ * other than 64 and 128, no layers or no heads). */
+uint64_t glacier_hip_kv4_page_bytes(uint32_t num_layers, uint32_t num_kv_heads, uint32_t head_dim);
+
+/* One step's pages, slots and rows from the lanes' lengths, on the device (the
+ * page map's arithmetic of paged_kv_cache.zig:1006-1072 without its
+ * ownership records), for pools of any element type with 16-position pages.
+ * Lane i has ctx_lens_dev[i] positions and takes new_rows_dev[i] more (either
+ * may be 0). Lanes in order take the pages they need for them from
+ * free_pages_dev[*free_taken_dev ..] in order, into their page-table entries;
+ * other entries stay. Written:
+ *   row_start_dev [lanes + 1]  first row of each lane, and the row count,
+ *   ctx_after_dev [lanes]      ctx + new (may be ctx_lens_dev itself),
+ *   slots_dev     [max_rows]   16 * page + position % 16 of each row,
+ *   row_lanes_dev, row_positions_dev [max_rows] (either may be NULL),
+ *   result_dev    [4]          {status, rows, pages taken, free entries taken
+ *                              so far}; free_taken_dev may be its last entry.
+ * Rows past the last one get slot, lane and position -1, and a row whose
+ * page-table entry is negative gets slot -1. A plan that does not hold --
+ * a negative length, more than max_rows rows (status SHAPE_MISMATCH), more
+ * positions than a table row or more pages than the free list has
+ * (CACHE_FULL) -- takes nothing: the table stays, ctx_after = ctx, no rows.
+ * lanes <= 1024, max_pages <= 2^26, no table larger than 2^31 entries.
+ * Asynchronous on `stream`; launches only. */
+int glacier_hip_kv_plan_rows(glacier_hip_context *ctx, const int32_t *ctx_lens_dev,
+                             const int32_t *new_rows_dev, uint32_t lanes, uint32_t max_rows,
+                             int32_t *page_table_dev, uint32_t max_pages,
+                             const int32_t *free_pages_dev, uint32_t free_count,
+                             const int32_t *free_taken_dev, int32_t *row_start_dev,
+                             int32_t *ctx_after_dev, int64_t *slots_dev, int32_t *row_lanes_dev,
+                             int32_t *row_positions_dev, int32_t *result_dev, void *stream);
+
+/* Quantise K and V rows into their slots (16 * page + position, as
+ * glacier_hip_kv_plan_rows gives them) of one layer. k_dev / v_dev hold rows
+ * of num_kv_heads * head_dim elements (kv_dtype F32, F16 or BF16), k_stride /
+ * v_stride elements apart, so both may be columns of one projection's output.
+ * Rows whose slot is negative or past the pool are skipped; the slots of one
+ * call must differ. Asynchronous on `stream`; launches only. */
+int glacier_hip_kv4_append(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool,
+                           uint32_t layer, const void *k_dev, const void *v_dev, int kv_dtype,
+                           uint64_t k_stride, uint64_t v_stride, const int64_t *slots_dev,
+                           uint32_t rows, void *stream);
+
+/* The stored values of slots of one layer, f32 [rows][num_kv_heads *
+ * head_dim], 16-byte aligned; rows whose slot is negative or past the pool
+ * are left as they were. Asynchronous on `stream`; launches only. */
+int glacier_hip_kv4_read(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool,
+                         uint32_t layer, const int64_t *slots_dev, uint32_t rows, float *k_dev,
+                         float *v_dev, void *stream);
+
+/* glacier_hip_paged_attention over 4-bit pages, for up to 1024 lanes: one
+ * query row per lane, softmax(q . K / sqrt(head_dim)) V over its
+ * ctx_lens_dev positions in f32 arithmetic on the stored values. A lane of
+ * length 0 gets zeros; a length outside 0..max_ctx, or a page id of an
+ * attended position outside the pool, makes the lane's output NaN.
+ * num_heads / num_kv_heads <= 8; max_ctx <= 16 * max_pages_per_lane; q_dev,
+ * out_dev (which must not overlap) and workspace_dev 16-byte aligned.
+ * workspace_dev holds glacier_hip_kv4_attention_workspace_bytes(lanes, lanes,
+ * num_heads, num_kv_heads, head_dim) bytes, zero before its first call; each
+ * call leaves it ready for the next. Calls that may overlap (streams, replays
+ * of two graphs) need a workspace each; a larger one serves smaller calls.
+ * Asynchronous on `stream`; launches only. */
+uint64_t glacier_hip_kv4_attention_workspace_bytes(uint32_t lanes, uint32_t max_rows,
+                                                   uint32_t num_heads, uint32_t num_kv_heads,
+                                                   uint32_t head_dim);
+int glacier_hip_paged_attention_kv4(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool,
+                                    uint32_t layer, const float *q_dev,
+                                    const int32_t *page_table_dev, uint32_t max_pages_per_lane,
+                                    const int32_t *ctx_lens_dev, uint32_t lanes,
+                                    uint32_t num_heads, uint32_t max_ctx, float *out_dev,
+                                    void *workspace_dev, uint64_t workspace_bytes, void *stream);
+
+/* The same for runs of rows (prompt chunks, drafted tokens and single tokens
+ * side by side): lane i's queries are rows row_start_dev[i] ..
+ * row_start_dev[i + 1] - 1 (as glacier_hip_kv_plan_rows gives them) at its
+ * last positions, so row r attends to positions 0 .. ctx_lens_dev[i] -
+ * row_start_dev[i + 1] + r, its own included; ctx_lens_dev counts the step's
+ * rows, whose K/V are already stored. Rows past the last lane's are left as
+ * they were; max_rows is the capacity of q_dev / out_dev. A lane with more
+ * rows than positions gets NaN, as the invalid lengths and pages above.
+ * Workspace for (lanes, max_rows). Asynchronous on `stream`; launches only. */
+int glacier_hip_paged_attention_kv4_rows(glacier_hip_context *ctx,
+                                         const glacier_hip_kv4_pool_t *pool, uint32_t layer,
+                                         const float *q_dev, const int32_t *page_table_dev,
+                                         uint32_t max_pages_per_lane, const int32_t *row_start_dev,
+                                         const int32_t *ctx_lens_dev, uint32_t lanes,
+                                         uint32_t max_rows, uint32_t num_heads, uint32_t max_ctx,
+                                         float *out_dev, void *workspace_dev,
+                                         uint64_t workspace_bytes, void *stream);
+
 /* ---- greedy samplers (sampling.zig:194-206, :55-105) ---------------------
  * rows independent logit rows of length n. Results are written to host
  * memory after the call synchronizes the stream. */
