@@ -10,6 +10,7 @@
 
 #include <algorithm>
 
+#include "int4_ops.h"
 #include "runtime.h"
 
 namespace gk {
@@ -336,6 +337,612 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Decode attention
+// ---------------------------------------------------------------------------
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;             // waves of a workgroup
+constexpr int kSplitPages = 2 * kWaves;   // fewest pages of a work item where a merge follows
+constexpr int kWholePages = 8 * kWaves;   // pages up to which a context stays one item
+constexpr int kTargetItems = 512;     // work items that share a long batch out
+constexpr float kSlack = 4.0f;        // log2 units a score may pass its reference before a rescale
+constexpr float kShift = 11.0f;       // log2 of a weight at the reference
+constexpr float kNoRef = -1e30f;      // the reference before the first score
+constexpr int kMaxRecords = 2 * kTargetItems + 2;
+
+static __device__ __forceinline__ v8h as_v8h(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const v4u w = {a, b, c, d};
+  return __builtin_bit_cast(v8h, w);
+}
+
+// Nibble N of both 16-bit halves of a word as halves (code - 8) * 2^-10, by
+// one packed fma of the code's bits (code * 2^-24, or 16 times that). Around
+// the middle of a group's range the products of a sum have both signs: an
+// MFMA takes its products to 2^-24 of the largest, towards zero, which for
+// products of one sign is a bias that the minima's part would not take out
+// again (2048 positions: 1e-4 of the output with codes of one sign). A
+// subnormal operand would count there as if it were 2^-14 (1e-5).
+template <int N>
+static __device__ __forceinline__ uint32_t mid_code(uint32_t w) {
+  const v2h c = __builtin_bit_cast(v2h, w & (N ? 0x00F000F0u : 0x000F000Fu));
+  const _Float16 k = N ? (_Float16)0x1p10f : (_Float16)0x1p14f, eight = (_Float16)-0x1p-7f;
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, v2h{k, k}, v2h{eight, eight}));
+}
+
+// Eight codes of a word, less 8: nibbles 0, 4, 1, 5, 2, 6, 3, 7.
+static __device__ __forceinline__ v8h mid_codes8(uint32_t w) {
+  const uint32_t u = w >> 8;
+  return as_v8h(mid_code<0>(w), mid_code<1>(w), mid_code<0>(u), mid_code<1>(u));
+}
+
+static __device__ __forceinline__ int wave_scan_dpp(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15 of rows 0, 2 onto 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31 onto the upper half
+  return v;
+}
+
+// The value of lane N of each 16-lane row.
+template <int N>
+static __device__ __forceinline__ float row_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + N, 0xF, 0xF, true));
+}
+
+// What a wave requests of two pages for one KV head.
+template <int HD>
+struct Pair {
+  static constexpr int NG = HD / 32;
+  uint32_t kc[2][NG], vc[2][NG];        // codes
+  uint32_t ks[2][2 * NG], vs[2][2 * NG];  // steps [g][4 positions]
+  uint32_t km[2][2 * NG];               // minima [4 positions][g]
+  uint32_t vo[2][2], vm[2][2];          // steps and minima of group j (lanes j < NG)
+};
+
+template <int N>
+static __device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_t *p) {
+  if constexpr (N == 1) {
+    d[0] = *(const uint32_t *)p;
+  } else if constexpr (N == 2) {
+    const uint2 v = *(const uint2 *)p;
+    d[0] = v.x;
+    d[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = *(const uint4 *)(p + 4 * i);
+      d[i] = v.x;
+      d[i + 1] = v.y;
+      d[i + 2] = v.z;
+      d[i + 3] = v.w;
+    }
+  }
+}
+
+template <int HD>
+static __device__ __forceinline__ void load_keys(Pair<HD> &b, const uint8_t *ta, const uint8_t *tb,
+                                                 int l) {
+  constexpr int NG = HD / 32;
+  const int c = l >> 4, j = l & 15;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const uint8_t *t = x ? tb : ta;
+    load_words(b.kc[x], t + j * (HD / 2) + c * (4 * NG));
+    load_words(b.ks[x], t + 8 * HD + c * (8 * NG));
+    load_words(b.km[x], t + 9 * HD + c * (8 * NG));
+  }
+}
+
+template <int HD>
+static __device__ __forceinline__ void load_values(Pair<HD> &b, const uint8_t *ta, const uint8_t *tb,
+                                                   int l) {
+  constexpr int NG = HD / 32, TILE = 10 * HD;
+  const int c = l >> 4, j = l & 15;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const uint8_t *t = (x ? tb : ta) + TILE;
+    load_words(b.vc[x], t + (c * 16 + j) * (4 * NG));
+    load_words(b.vs[x], t + 8 * HD + c * (8 * NG));
+    load_words(b.vo[x], t + 8 * HD + c * (8 * NG) + min(j, NG - 1) * 8);
+    load_words(b.vm[x], t + 9 * HD + c * (8 * NG) + min(j, NG - 1) * 8);
+  }
+}
+
+// Steps and minima of positions from n on (of 32) become zero: a stale page
+// may hold anything there.
+static __device__ __forceinline__ void masks_of(int left, uint32_t &lo, uint32_t &hi) {
+  lo = left > 1 ? 0xFFFFFFFFu : left > 0 ? 0xFFFFu : 0u;
+  hi = left > 3 ? 0xFFFFFFFFu : left > 2 ? 0xFFFFu : 0u;
+}
+template <int HD>
+static __device__ __forceinline__ void cut_keys(Pair<HD> &b, int n, int l) {
+  constexpr int NG = HD / 32;
+  const int c = l >> 4;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    uint32_t lo, hi;
+    masks_of(n - 16 * x - 4 * c, lo, hi);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      b.ks[x][2 * g] &= lo;
+      b.ks[x][2 * g + 1] &= hi;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i)
+      if (4 * c + 2 * i / NG >= n - 16 * x) b.km[x][i] = 0u;
+  }
+}
+template <int HD>
+static __device__ __forceinline__ void cut_values(Pair<HD> &b, int n, int l) {
+  constexpr int NG = HD / 32;
+  const int c = l >> 4;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    uint32_t lo, hi;
+    masks_of(n - 16 * x - 4 * c, lo, hi);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      b.vs[x][2 * g] &= lo;
+      b.vs[x][2 * g + 1] &= hi;
+    }
+    b.vo[x][0] &= lo;
+    b.vo[x][1] &= hi;
+    b.vm[x][0] &= lo;
+    b.vm[x][1] &= hi;
+  }
+}
+
+// The larger of each two halves (as integers: halves that are not negative).
+static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u2, a), __builtin_bit_cast(u2, b)));
+}
+
+static __device__ __forceinline__ float half_of(uint32_t w, int hi) {
+  return (float)__builtin_bit_cast(v2h, w)[hi];
+}
+
+// fp16 of x, or with low = 1 of what that leaves of x. x is a rounded f32 on
+// both sides: the compiler would otherwise round the product that made it
+// straight to fp16 on one of them, and where the two roundings differ the
+// parts do not add up to x.
+static __device__ __forceinline__ _Float16 half_part(float x, float low) {
+  asm("" : "+v"(x));
+  const _Float16 h = (_Float16)x;
+  return (_Float16)fmaf(-(float)h, low, x);
+}
+
+// A wave's running state for the query heads of one KV head. Lanes (c, j) =
+// 16 c + j: columns j and j + 8 are one query head's fp16 high and low parts.
+template <int HD>
+struct Wave {
+  v8h q[HD / 32];       // query operands, a group a step
+  float qsum[HD / 32];  // sums of q over each group, in the high parts' columns
+  float mult;      // log2 units of a score's accumulator unit, a power of two
+  f4 o[HD / 16];   // rows: heads (high, then low parts), columns: dims 16 e + j
+  f4 om;           // the minima's part, columns: groups
+  float ref;       // log2 units of the head's reference score
+  float sum;       // weights of this lane's positions
+  int e;           // V steps are below 2^e
+  uint32_t bound;  // 2^e as two halves
+};
+
+// New reference of scores that passed the old one by kSlack, or a new bound
+// of the V steps: what was summed so far follows. v: scores before mult.
+template <int HD>
+static __device__ __forceinline__ void raise(Wave<HD> &s, const float (&v)[8], const uint32_t (&steps)[2][2], int l) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, v[i] * s.mult);
+  top = xor32_max(xor16_max(top));  // same in both columns of a head
+  const float ref = top - s.ref > kSlack ? top : s.ref, f = exp2f(s.ref - ref);
+  s.ref = ref;
+  s.sum *= f;
+  // steps that are no NaN, as integers in their order
+  int big = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int a = (int)(steps[i >> 2][i >> 1 & 1] >> 16 * (i & 1) & 0x7FFFu);
+    if (a < 0x7C00) big = max(big, a);
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) big = max(big, __shfl_xor(big, m, 64));
+  const int old = s.e;
+  const int e = big >> 10 == 0 ? -14 : (big >> 10) - 14;  // below 2^e
+  s.e = max(old, e);
+  s.bound = (uint32_t)(s.e + 15) << 10;
+  s.bound |= s.bound << 16;
+  const float g = ldexpf(1.0f, old - s.e);
+  const int c = l >> 4;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float fr = __shfl(f, (4 * c + r) & 7, 64);
+    s.om[r] *= fr;
+#pragma unroll
+    for (int e2 = 0; e2 < HD / 16; ++e2) s.o[e2][r] *= fr * g;
+  }
+}
+
+// Scores of n positions (of 32) of a pair, in units that mult takes to log2:
+// lane (c, j) has positions 4 c + r of both pages for column j.
+template <int HD>
+static __device__ __forceinline__ void scores(const Wave<HD> &s, Pair<HD> &b, int n, int l, float (&v)[8]) {
+  constexpr int NG = HD / 32;
+  const int c = l >> 4;
+  if (n < 32) cut_keys(b, n, l);
+  const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    f4 sc = zero;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(mid_codes8(b.kc[x][g]), s.q[g], zero, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float step = half_of(b.ks[x][2 * g + (r >> 1)], r & 1);
+        const float mid = fmaf(8.0f, step, half_of(b.km[x][(r * NG + g) >> 1], g & 1));
+        sc[r] = fmaf(step, acc[r], fmaf(mid, s.qsum[g], sc[r]));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[4 * x + r] = sc[r] + row_xor8(sc[r]);  // high and low parts of the query
+  }
+  if (n < 32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (16 * (i >> 2) + 4 * c + (i & 3) >= n) v[i] = -INFINITY;
+  }
+}
+
+// Adds the pair's values with those scores to the state.
+template <int HD>
+static __device__ __forceinline__ void weigh(Wave<HD> &s, Pair<HD> &b, int n, int l, const float (&v)[8]) {
+  constexpr int NG = HD / 32, NH = HD / 64;
+  const int j = l & 15;
+  if (n < 32) cut_values(b, n, l);
+  const float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])),
+                          fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+  const bool over = max2(max2(max2(b.vo[0][0], b.vo[0][1]), max2(b.vo[1][0], b.vo[1][1])), s.bound) != s.bound;
+  if (__any(fmaf(top, s.mult, -s.ref) > kSlack || over)) raise(s, v, b.vo, l);
+  const float unit = ldexpf(1.0f, -s.e), low = j < 8 ? 0.0f : 1.0f;
+  const float shift = kShift - s.ref;
+  float p[8], pu[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(fmaf(v[i], s.mult, shift));
+    s.sum += p[i];
+    pu[i] = p[i] * unit;
+  }
+  auto part = [&](const float (&x)[8]) {
+    v8h a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = half_part(x[i], low);
+    return a;
+  };
+  v8h mid, rest;  // the middle of group j's range, code 8, in two parts
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int x = i >> 2, y = (i & 3) >> 1;
+    const float m = fmaf(8.0f, half_of(b.vo[x][y], i & 1), half_of(b.vm[x][y], i & 1));
+    mid[i] = (_Float16)m;
+    rest[i] = (_Float16)(m - (float)mid[i]);
+  }
+  const v8h pp = part(p);
+  s.om = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp, mid, s.om, 0, 0, 0);
+  s.om = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp, rest, s.om, 0, 0, 0);
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] = half_of(b.vs[i >> 2][2 * g + ((i & 3) >> 1)], i & 1) * pu[i];
+    const v8h a = part(x);
+    // blocks 2 g, 2 g + 1: nibbles 2 (g % 2), + 1 of the words of unit g / 2
+    const int h = g >> 1, sh = 8 * (g & 1);
+    const uint32_t w[4] = {b.vc[0][h] >> sh, b.vc[0][NH + h] >> sh, b.vc[1][h] >> sh,
+                           b.vc[1][NH + h] >> sh};
+    s.o[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+        a, as_v8h(mid_code<0>(w[0]), mid_code<0>(w[1]), mid_code<0>(w[2]), mid_code<0>(w[3])),
+        s.o[2 * g], 0, 0, 0);
+    s.o[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+        a, as_v8h(mid_code<1>(w[0]), mid_code<1>(w[1]), mid_code<1>(w[2]), mid_code<1>(w[3])),
+        s.o[2 * g + 1], 0, 0, 0);
+  }
+}
+
+// The query operands of one row's heads: q log2(e) / sqrt(HD) = 2^e q', the
+// largest |q'| of a head in [2^13, 2^14), split into fp16 high and low parts.
+template <int HD>
+static __device__ __forceinline__ void load_query(Wave<HD> &s, const float *q, int G, int l) {
+  constexpr int NG = HD / 32;
+  const int c = l >> 4, j = l & 15, head = j & 7;
+  const float unit = 1.44269504088896341f / sqrtf((float)HD);
+  float v[NG][8];
+  float top = 0.0f;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const float *p = q + (size_t)(head < G ? head : 0) * HD + 32 * g + 8 * c;
+    const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
+    const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[g][i] = head < G ? w[i] * unit : 0.0f;
+      top = fmaxf(top, fabsf(v[g][i]));
+    }
+  }
+  top = xor32_max(xor16_max(top));
+  const int e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+  s.mult = ldexpf(1.0f, e + 10);
+  const float low = j < 8 ? 0.0f : 1.0f;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[g][i] = ldexpf(v[g][i], -e);
+      sum += v[g][i];
+    }
+    sum = xor32_add(xor16_add(sum));
+    s.qsum[g] = j < 8 ? sum * 0x1p-10f : 0.0f;  // (codes come times 2^-10)
+    constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};  // of mid_codes8
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      s.q[g][i] = half_part(v[g][order[i]], low);
+    }
+  }
+}
+
+template <int HD>
+struct DecodeLds {
+  float o[kWaves][kMaxGroup][HD];
+  float ref[kWaves][kMaxGroup], sum[kWaves][kMaxGroup];
+  int scan[kWaves], item[6];
+};
+
+struct MergeItem {  // of a (lane, KV head): its chunks' records
+  int start, pages, chunks, half;
+};
+// First page of chunk ch, and its record: the place of its first page in the
+// batch divided by half the most pages of a chunk.
+static __device__ __forceinline__ int chunk_first(int ch, int pages, int chunks) {
+  return ch * (pages / chunks) + min(ch, pages % chunks);
+}
+
+// Work items: (lane, KV head, chunk of its pages). Q, the most pages of a
+// chunk, comes from the batch's own lengths: about kTargetItems items share
+// it out, `least` pages each at least. The chunks of a lane are of equal size to a page, so
+// where there are several they hold Q / 2 pages at least.
+template <int HD>
+__global__ __launch_bounds__(64 * kWaves, 2) void kv4_decode_kernel(AttnArgs a, int least,
+                                                                 MergeItem *merge, float *records) {
+  __shared__ DecodeLds<HD> s;
+  const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int c = l >> 4, j = l & 15;
+  const int Hkv = a.kv.heads, G = a.num_heads / Hkv;
+  const float nan = __uint_as_float(0x7FC00000u);
+
+  // the lanes' pages: a thread holds `per` lanes
+  const int per = (a.lanes + 64 * kWaves - 1) / (64 * kWaves);
+  int pages[4], mine = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = t * per + i;
+    const int n = i < per && at < a.lanes ? a.ctx[at] : 0;
+    pages[i] = n > 0 && n <= a.max_ctx ? (n + kPage - 1) / kPage : 0;
+    mine += pages[i];
+  }
+  const int pages_in = wave_scan_dpp(mine);
+  if (l == 63) s.scan[w] = pages_in;
+  __syncthreads();
+  int total = 0, pages_before = pages_in - mine;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < w) pages_before += s.scan[i];
+    total += s.scan[i];
+  }
+  __syncthreads();
+  // (even, so that half of it is whole)
+  const int Q = (max(least, (total * Hkv + kTargetItems - 1) / kTargetItems) + 1) & ~1;
+  int items = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) items += (pages[i] + Q - 1) / Q * Hkv;
+  const int items_in = wave_scan_dpp(items);
+  if (l == 63) s.scan[w] = items_in;
+  __syncthreads();
+  int all = 0, items_before = items_in - items;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < w) items_before += s.scan[i];
+    all += s.scan[i];
+  }
+
+  // a lane without positions, or with a length that does not hold
+  if ((int)blockIdx.x < a.lanes) {
+    const int n = a.ctx[blockIdx.x];
+    if (n <= 0 || n > a.max_ctx) {
+      for (int i = t; i < a.num_heads * HD; i += 64 * kWaves)
+        a.out[(size_t)blockIdx.x * a.num_heads * HD + i] = n == 0 ? 0.0f : nan;
+      if (merge)
+        for (int i = t; i < Hkv; i += 64 * kWaves) merge[blockIdx.x * Hkv + i].chunks = 0;
+    }
+  }
+  const int item = blockIdx.x;
+  if (item >= all) return;
+  if (item >= items_before && item < items_before + items) {
+    int at = items_before, pb = pages_before;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int chunks = (pages[i] + Q - 1) / Q, r = item - at;
+      if (r >= 0 && r < chunks * Hkv) {
+        s.item[0] = t * per + i;
+        s.item[1] = r / chunks;
+        s.item[2] = r % chunks;
+        s.item[3] = chunks;
+        s.item[4] = pages[i];
+        s.item[5] = pb * Hkv + r / chunks * pages[i];
+      }
+      at += chunks * Hkv;
+      pb += pages[i];
+    }
+  }
+  __syncthreads();
+  const int lane = __builtin_amdgcn_readfirstlane(s.item[0]), h = __builtin_amdgcn_readfirstlane(s.item[1]);
+  const int ch = __builtin_amdgcn_readfirstlane(s.item[2]), chunks = __builtin_amdgcn_readfirstlane(s.item[3]);
+  const int lane_pages = __builtin_amdgcn_readfirstlane(s.item[4]), start = __builtin_amdgcn_readfirstlane(s.item[5]);
+  const int first = chunk_first(ch, lane_pages, chunks), end = chunk_first(ch + 1, lane_pages, chunks);
+  const int ctx = __builtin_amdgcn_readfirstlane(a.ctx[lane]);
+  if (merge && ch == 0 && t == 0) merge[lane * Hkv + h] = {start, lane_pages, chunks, Q / 2};
+
+  Wave<HD> s_w;
+#pragma unroll
+  for (int e = 0; e < HD / 16; ++e) s_w.o[e] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  s_w.om = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  s_w.ref = kNoRef;
+  s_w.sum = 0.0f;
+  s_w.e = -14;
+  s_w.bound = 1u << 10 | 1u << 26;
+  load_query(s_w, a.q + ((size_t)lane * a.num_heads + h * G) * HD, G, l);
+
+  // a wave takes pairs of pages w, w + kWaves, ... of the chunk
+  const int32_t *table = a.table + (size_t)lane * a.max_pages;
+  const uint8_t *head_base = a.kv.base + (size_t)(2 * h) * (10 * HD);
+  int bad = 0;
+  const int stop = min(ctx, end * kPage);
+  for (int p0 = first + 2 * w; p0 < end; p0 += 64 * kWaves) {
+    // ids of the next 32 pairs, two lanes a pair (a page past the chunk: its first one)
+    const int at = p0 + (l >> 1) * (2 * kWaves) + (l & 1);
+    uint32_t id = (uint32_t)table[at < end ? at : first];
+    if (id >= a.kv.page_count) {
+      bad = 1;
+      id = 0;
+    }
+    const int n = min(32, (end - p0 + 2 * kWaves - 1) / (2 * kWaves));  // pairs
+    auto tile = [&](int i, int x) {
+      return head_base + (size_t)(uint32_t)__builtin_amdgcn_readlane((int)id, 2 * i + x) * a.kv.page_bytes;
+    };
+    Pair<HD> b;
+    load_keys(b, tile(0, 0), tile(0, 1), l);
+    load_values(b, tile(0, 0), tile(0, 1), l);
+    for (int i = 0; i < n; ++i) {
+      // the next pair's keys are requested once this one's are used up, and its values
+      // after these; past the last pair they are requested again and not used
+      const int next = min(i + 1, n - 1), left = min(32, stop - (p0 + i * 2 * kWaves) * kPage);
+      const uint8_t *ta = tile(next, 0), *tb = tile(next, 1);
+      float x[8];
+      scores(s_w, b, left, l, x);
+      load_keys(b, ta, tb, l);
+      weigh(s_w, b, left, l, x);
+      load_values(b, ta, tb, l);
+    }
+  }
+
+  // the waves' states, then their sums weighted by 2^(reference - the largest)
+  const float unit = ldexpf(1.0f, s_w.e + 10);
+  float om[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) om[r] = xor32_add(s_w.om[r]);
+#pragma unroll
+  for (int e = 0; e < HD / 16; ++e)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float m = e / 2 == 0 ? row_lane<0>(om[r]) : e / 2 == 1 ? row_lane<1>(om[r])
+                      : e / 2 == 2 ? row_lane<2>(om[r]) : row_lane<3>(om[r]);
+      const float v = fmaf(xor32_add(s_w.o[e][r]), unit, m);
+      if (c < 2) s.o[w][4 * c + r][16 * e + j] = v;
+    }
+  const float sum = xor32_add(xor16_add(s_w.sum));
+  if (l < kMaxGroup) {
+    s.ref[w][l] = s_w.ref;
+    s.sum[w][l] = sum;
+  }
+  bad = __syncthreads_or(bad);
+  float *rec = records + (size_t)((start + first) / (Q / 2)) * (kMaxGroup * (HD + 2));
+  for (int i = t; i < G * HD; i += 64 * kWaves) {
+    const int g = i / HD, d = i % HD;
+    float top = s.ref[0][g];
+#pragma unroll
+    for (int v = 1; v < kWaves; ++v) top = fmaxf(top, s.ref[v][g]);
+    float L = 0.0f, O = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float f = __builtin_amdgcn_exp2f(s.ref[v][g] - top);
+      L = fmaf(s.sum[v][g], f, L);
+      O = fmaf(s.o[v][g][d], f, O);
+    }
+    if (bad) L = nan;
+    if (chunks == 1) {
+      a.out[((size_t)lane * a.num_heads + h * G + g) * HD + d] = O / L;
+    } else {
+      rec[g * (HD + 2) + 2 + d] = O;
+      if (d == 0) {
+        rec[g * (HD + 2)] = top;
+        rec[g * (HD + 2) + 1] = L;
+      }
+    }
+  }
+}
+
+// The chunks of a (lane, query head) added up, weighted by 2^(reference - the
+// largest): HD / 4 threads a record, in a fixed order.
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, const MergeItem *merge,
+                                                        const float *records) {
+  constexpr int TPR = HD / 4, R = 256 / TPR;  // threads a record, records at a time
+  __shared__ float f_s[kMaxRecords];
+  __shared__ float4 o_s[R][TPR];
+  __shared__ float wave_s[2][4];
+  const int t = threadIdx.x, l = t & 63, w = t >> 6;
+  const int lane = blockIdx.x / a.num_heads, qh = blockIdx.x % a.num_heads;
+  const int G = a.num_heads / a.kv.heads, g = qh % G;
+  const MergeItem m = merge[lane * a.kv.heads + qh / G];
+  if (m.chunks <= 1) return;
+  auto rec = [&](int ch) {
+    return records + ((size_t)((m.start + chunk_first(ch, m.pages, m.chunks)) / m.half) * kMaxGroup + g) * (HD + 2);
+  };
+  float top = -INFINITY;
+  for (int ch = t; ch < m.chunks; ch += 256) {
+    f_s[ch] = rec(ch)[0];
+    top = fmaxf(top, f_s[ch]);
+  }
+  top = wave_max(top);
+  if (l == 0) wave_s[0][w] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(wave_s[0][0], wave_s[0][1]), fmaxf(wave_s[0][2], wave_s[0][3]));
+  float sum = 0.0f;
+  for (int ch = t; ch < m.chunks; ch += 256) {
+    const float f = __builtin_amdgcn_exp2f(f_s[ch] - top);
+    f_s[ch] = f;
+    sum = fmaf(rec(ch)[1], f, sum);
+  }
+  sum = wave_sum(sum);
+  if (l == 0) wave_s[1][w] = sum;
+  __syncthreads();
+  sum = (wave_s[1][0] + wave_s[1][1]) + (wave_s[1][2] + wave_s[1][3]);
+  const int rw = t / TPR, d = t % TPR * 4;
+  float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int ch = rw; ch < m.chunks; ch += R) {
+    const float *p = rec(ch) + 2 + d;
+    const float f = f_s[ch];
+    const float2 x = *(const float2 *)p, y = *(const float2 *)(p + 2);
+    o.x = fmaf(x.x, f, o.x);
+    o.y = fmaf(x.y, f, o.y);
+    o.z = fmaf(y.x, f, o.z);
+    o.w = fmaf(y.y, f, o.w);
+  }
+  o_s[rw][t % TPR] = o;
+  __syncthreads();
+  if (t < HD) {
+    float v = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) v += ((const float *)&o_s[r][t / 4])[t % 4];
+    a.out[((size_t)lane * a.num_heads + qh) * HD + t] = v / sum;
+  }
+}
+
 }  // namespace
 }  // namespace gk
 
@@ -380,6 +987,10 @@ int pool_view(const glacier_hip_kv4_pool_t *p, uint32_t layer, gk::Kv4 *out) {
   return GLACIER_HIP_OK;
 }
 
+size_t kMergeBytes(uint32_t lanes, uint32_t heads) {
+  return ((size_t)lanes * heads * sizeof(gk::MergeItem) + 255) & ~(size_t)255;
+}
+
 int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint32_t layer,
               const float *q, const int32_t *table, uint32_t max_pages, const int32_t *row_start,
               const int32_t *lens, uint32_t lanes, uint32_t max_rows, uint32_t num_heads,
@@ -392,7 +1003,8 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
   const uint64_t need = glacier_hip_kv4_attention_workspace_bytes(lanes, max_rows, num_heads,
                                                                   pool->num_kv_heads, pool->head_dim);
   if (need == 0 || ws_bytes < need || max_ctx == 0 || max_ctx > (1u << 30) ||
-      max_ctx > (uint64_t)max_pages * gk::kPage)
+      max_ctx > (uint64_t)max_pages * gk::kPage ||
+      (uint64_t)lanes * ((max_ctx + 15) / 16) * pool->num_kv_heads >= (1ull << 31))
     return GLACIER_HIP_SHAPE_MISMATCH;
   a.q = q;
   a.table = table;
@@ -408,6 +1020,26 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
   DeviceScope on(ctx->device);
   GH_CHECK(ctx, on.err);
   hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
+  if (!row_start) {
+    // a merge follows where a context may be more than one item
+    const bool split = (max_ctx + gk::kPage - 1) / gk::kPage > (uint32_t)gk::kWholePages;
+    const int least = split ? gk::kSplitPages : gk::kWholePages;
+    auto *merge = split ? (gk::MergeItem *)ws : nullptr;
+    float *records = (float *)((char *)ws + kMergeBytes(lanes, pool->num_kv_heads));
+    const uint64_t each = ((max_ctx + gk::kPage - 1) / gk::kPage + least - 1) / least;
+    const uint32_t items = (uint32_t)std::min<uint64_t>(
+        (uint64_t)lanes * a.kv.heads * each, (uint64_t)lanes * a.kv.heads + gk::kTargetItems);
+    const uint32_t grid = std::max(items, lanes);
+    if (pool->head_dim == 128) {
+      gk::kv4_decode_kernel<128><<<grid, 64 * gk::kWaves, 0, st>>>(a, least, merge, records);
+      if (split) gk::kv4_merge_kernel<128><<<lanes * num_heads, 256, 0, st>>>(a, merge, records);
+    } else {
+      gk::kv4_decode_kernel<64><<<grid, 64 * gk::kWaves, 0, st>>>(a, least, merge, records);
+      if (split) gk::kv4_merge_kernel<64><<<lanes * num_heads, 256, 0, st>>>(a, merge, records);
+    }
+    GH_CHECK(ctx, hipGetLastError());
+    return GLACIER_HIP_OK;
+  }
   const dim3 grid(max_rows, pool->num_kv_heads);
   if (pool->head_dim == 128) gk::kv4_attn_kernel<128><<<grid, 256, 0, st>>>(a);
   else gk::kv4_attn_kernel<64><<<grid, 256, 0, st>>>(a);
@@ -523,7 +1155,8 @@ uint64_t glacier_hip_kv4_attention_workspace_bytes(uint32_t lanes, uint32_t max_
       num_heads % num_kv_heads != 0 || num_heads / num_kv_heads == 0 ||
       num_heads / num_kv_heads > (uint32_t)gk::kMaxGroup)
     return 0;
-  return 256;
+  return kMergeBytes(lanes, num_kv_heads) +
+         (uint64_t)gk::kMaxRecords * gk::kMaxGroup * (head_dim + 2) * sizeof(float);
 }
 
 int glacier_hip_paged_attention_kv4(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool,
