@@ -344,37 +344,38 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;             // waves of a workgroup
+constexpr int kRing = 2;              // pairs of pages a wave has on their way
 constexpr int kSplitPages = 2 * kWaves;   // fewest pages of a work item where a merge follows
 constexpr int kWholePages = 8 * kWaves;   // pages up to which a context stays one item
-constexpr int kTargetItems = 512;     // work items that share a long batch out
+constexpr int kMaxSlots = 1024;       // workgroups that a batch is cut for, at most
 constexpr float kSlack = 4.0f;        // log2 units a score may pass its reference before a rescale
 constexpr float kShift = 11.0f;       // log2 of a weight at the reference
 constexpr float kNoRef = -1e30f;      // the reference before the first score
-constexpr int kMaxRecords = 2 * kTargetItems + 2;
+constexpr int kMaxRecords = 4 * kMaxSlots + 2;
 
 static __device__ __forceinline__ v8h as_v8h(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   const v4u w = {a, b, c, d};
   return __builtin_bit_cast(v8h, w);
 }
 
-// Nibble N of both 16-bit halves of a word as halves (code - 8) * 2^-10, by
-// one packed fma of the code's bits (code * 2^-24, or 16 times that). Around
-// the middle of a group's range the products of a sum have both signs: an
-// MFMA takes its products to 2^-24 of the largest, towards zero, which for
-// products of one sign is a bias that the minima's part would not take out
-// again (2048 positions: 1e-4 of the output with codes of one sign). A
-// subnormal operand would count there as if it were 2^-14 (1e-5).
-template <int N>
-static __device__ __forceinline__ uint32_t mid_code(uint32_t w) {
+// Nibble N of both 16-bit halves of a word as halves (code - mid) * 2^-10, by
+// one packed operation on the code's bits (code * 2^-24, or 16 times that).
+// An MFMA takes the products of each eight k to 2^-24 of the largest, towards
+// zero, and counts a subnormal operand as 2^-14 there: codes left at 2^-24
+// cost 1e-5 of the output. V codes go around the middle of their range, 8:
+// products of one sign would be cut by a bias that the minima's part does not
+// take out again (1e-4 at 2048 positions); with K the query has both signs.
+template <int N, bool kMid>
+static __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
   const v2h c = __builtin_bit_cast(v2h, w & (N ? 0x00F000F0u : 0x000F000Fu));
-  const _Float16 k = N ? (_Float16)0x1p10f : (_Float16)0x1p14f, eight = (_Float16)-0x1p-7f;
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, v2h{k, k}, v2h{eight, eight}));
+  const _Float16 k = N ? (_Float16)0x1p10f : (_Float16)0x1p14f, mid = (_Float16)-0x1p-7f;
+  return __builtin_bit_cast(uint32_t, kMid ? __builtin_elementwise_fma(c, v2h{k, k}, v2h{mid, mid}) : c * v2h{k, k});
 }
 
-// Eight codes of a word, less 8: nibbles 0, 4, 1, 5, 2, 6, 3, 7.
-static __device__ __forceinline__ v8h mid_codes8(uint32_t w) {
+// Eight K codes of a word: nibbles 0, 4, 1, 5, 2, 6, 3, 7.
+static __device__ __forceinline__ v8h codes8(uint32_t w) {
   const uint32_t u = w >> 8;
-  return as_v8h(mid_code<0>(w), mid_code<1>(w), mid_code<0>(u), mid_code<1>(u));
+  return as_v8h(code_pair<0, false>(w), code_pair<1, false>(w), code_pair<0, false>(u), code_pair<1, false>(u));
 }
 
 static __device__ __forceinline__ int wave_scan_dpp(int v) {
@@ -399,8 +400,8 @@ struct Pair {
   static constexpr int NG = HD / 32;
   uint32_t kc[2][NG], vc[2][NG];        // codes
   uint32_t ks[2][2 * NG], vs[2][2 * NG];  // steps [g][4 positions]
-  uint32_t km[2][2 * NG];               // minima [4 positions][g]
-  uint32_t vo[2][2], vm[2][2];          // steps and minima of group j (lanes j < NG)
+  uint32_t km[2][NG / 2];               // minima of position j
+  uint32_t vo[2][2], vm[2][2];          // steps and minima of group j (j = NG: a group of ones)
 };
 
 template <int N>
@@ -423,32 +424,88 @@ static __device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_
   }
 }
 
+// Pairs of pages come through LDS: a wave copies them straight there, kRing
+// pairs ahead of the one it works on, each in loads of 16 bytes a lane, and
+// reads its operands from its own ring. (Registers hold one pair more than
+// the one in use at most, and the latency of a loaded memory takes three.)
+// A slot: K codes of both pages in lane order, V codes, then each page's K
+// steps, K minima, V steps, V minima.
 template <int HD>
-static __device__ __forceinline__ void load_keys(Pair<HD> &b, const uint8_t *ta, const uint8_t *tb,
-                                                 int l) {
-  constexpr int NG = HD / 32;
-  const int c = l >> 4, j = l & 15;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const uint8_t *t = x ? tb : ta;
-    load_words(b.kc[x], t + j * (HD / 2) + c * (4 * NG));
-    load_words(b.ks[x], t + 8 * HD + c * (8 * NG));
-    load_words(b.km[x], t + 9 * HD + c * (8 * NG));
+struct Slot {
+  static constexpr int kCodes = 8 * HD, kMeta = 2 * HD;  // bytes of a tile's codes, steps and minima
+  uint8_t kc[2][kCodes], vc[2][kCodes], meta[2][2 * kMeta];
+  uint16_t one[8];  // four steps 0 and four minima 1: a group of ones
+};
+// Loads of a pair (each counts one in vmcnt).
+template <int HD>
+constexpr int kPairLoads = HD == 128 ? 5 : 3;
+
+// 16 bytes a lane from p (+ off, p the wave's) to LDS base + 16 * lane (M0, which the compiler
+// keeps nothing in). The compiler does not see these loads: with its own
+// builtin every LDS read waits for all of them. arrive() waits for them, and
+// no other wait gets shorter by them (vector memory operations complete in
+// order).
+static __device__ __forceinline__ void copy16(uint32_t base, const uint8_t *p, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(base), "v"(off), "s"(p)
+               : "memory");
+}
+static __device__ __forceinline__ void copy16(uint32_t base, const uint8_t *p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p)
+               : "memory");
+}
+template <int N>
+static __device__ __forceinline__ void arrive() {  // all but the last N vector memory operations
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+template <int HD>
+static __device__ __forceinline__ void copy_pair(Slot<HD> *slot, const uint8_t *ta, const uint8_t *tb, int l) {
+  constexpr int TILE = 10 * HD;
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)slot;
+  // the slot's last reads are done
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  if constexpr (HD == 128) {
+    const int kc = ((l & 15) * 4 + (l >> 4)) * 16;  // lane (c, j): chunk c of position j
+    copy16(at, ta, kc);
+    copy16(at + 1024, tb, kc);
+    copy16(at + 2048, ta, TILE + l * 16);
+    copy16(at + 3072, tb, TILE + l * 16);
+    const int m = l & 31;
+    copy16(at + 4096, (l < 32 ? ta : tb) + (m < 16 ? 8 * HD : TILE + 8 * HD) + (m & 15) * 16);
+  } else {
+    const uint8_t *t = l < 32 ? ta : tb;
+    const int m = l & 31;
+    copy16(at, t + m * 16);
+    copy16(at + 1024, t + TILE + m * 16);
+    const int x = l & 15;
+    if (l < 32) copy16(at + 2048, (l < 16 ? ta : tb) + (x < 8 ? 8 * HD : TILE + 8 * HD) + (x & 7) * 16);
   }
 }
 
 template <int HD>
-static __device__ __forceinline__ void load_values(Pair<HD> &b, const uint8_t *ta, const uint8_t *tb,
-                                                   int l) {
-  constexpr int NG = HD / 32, TILE = 10 * HD;
+static __device__ __forceinline__ void read_keys(Pair<HD> &b, const Slot<HD> *s, int l) {
+  constexpr int NG = HD / 32;
   const int c = l >> 4, j = l & 15;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    const uint8_t *t = (x ? tb : ta) + TILE;
-    load_words(b.vc[x], t + (c * 16 + j) * (4 * NG));
-    load_words(b.vs[x], t + 8 * HD + c * (8 * NG));
-    load_words(b.vo[x], t + 8 * HD + c * (8 * NG) + min(j, NG - 1) * 8);
-    load_words(b.vm[x], t + 9 * HD + c * (8 * NG) + min(j, NG - 1) * 8);
+    load_words(b.kc[x], s->kc[x] + (HD == 128 ? l * 16 : j * 32 + c * 8));
+    load_words(b.ks[x], s->meta[x] + c * (8 * NG));
+    load_words(b.km[x], s->meta[x] + HD + j * (2 * NG));
+  }
+}
+
+template <int HD>
+static __device__ __forceinline__ void read_values(Pair<HD> &b, const Slot<HD> *s, int l) {
+  constexpr int NG = HD / 32;
+  const int c = l >> 4, j = l & 15;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const uint8_t *t = s->meta[x] + 2 * HD;
+    load_words(b.vc[x], s->vc[x] + l * (4 * NG));
+    load_words(b.vs[x], t + c * (8 * NG));
+    const uint8_t *one = (const uint8_t *)s->one, *o = t + c * (8 * NG) + min(j, NG - 1) * 8;
+    load_words(b.vo[x], j == NG ? one : o);
+    load_words(b.vm[x], j == NG ? one + 8 : o + HD);
   }
 }
 
@@ -461,7 +518,7 @@ static __device__ __forceinline__ void masks_of(int left, uint32_t &lo, uint32_t
 template <int HD>
 static __device__ __forceinline__ void cut_keys(Pair<HD> &b, int n, int l) {
   constexpr int NG = HD / 32;
-  const int c = l >> 4;
+  const int c = l >> 4, j = l & 15;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     uint32_t lo, hi;
@@ -472,8 +529,7 @@ static __device__ __forceinline__ void cut_keys(Pair<HD> &b, int n, int l) {
       b.ks[x][2 * g + 1] &= hi;
     }
 #pragma unroll
-    for (int i = 0; i < 2 * NG; ++i)
-      if (4 * c + 2 * i / NG >= n - 16 * x) b.km[x][i] = 0u;
+    for (int i = 0; i < NG / 2; ++i) b.km[x][i] = j < n - 16 * x ? b.km[x][i] : 0u;
   }
 }
 template <int HD>
@@ -506,14 +562,16 @@ static __device__ __forceinline__ float half_of(uint32_t w, int hi) {
   return (float)__builtin_bit_cast(v2h, w)[hi];
 }
 
-// fp16 of x, or with low = 1 of what that leaves of x. x is a rounded f32 on
-// both sides: the compiler would otherwise round the product that made it
-// straight to fp16 on one of them, and where the two roundings differ the
-// parts do not add up to x.
-static __device__ __forceinline__ _Float16 half_part(float x, float low) {
-  asm("" : "+v"(x));
-  const _Float16 h = (_Float16)x;
-  return (_Float16)fmaf(-(float)h, low, x);
+// fp16 of x and y, or with low = 1 of what that leaves of them. Both sides
+// round the f32 value: the compiler would otherwise round the product that
+// made it straight to fp16 on one of them, and where the two roundings differ
+// the parts do not add up.
+static __device__ __forceinline__ v2h half_parts(float x, float y, float low) {
+  asm("" : "+v"(x), "+v"(y));
+  uint32_t h = __builtin_bit_cast(uint32_t, v2h{(_Float16)x, (_Float16)y});
+  asm("" : "+v"(h));  // one conversion for the two
+  const v2h p = __builtin_bit_cast(v2h, h);
+  return v2h{(_Float16)fmaf(-(float)p.x, low, x), (_Float16)fmaf(-(float)p.y, low, y)};
 }
 
 // A wave's running state for the query heads of one KV head. Lanes (c, j) =
@@ -521,12 +579,11 @@ static __device__ __forceinline__ _Float16 half_part(float x, float low) {
 template <int HD>
 struct Wave {
   v8h q[HD / 32];       // query operands, a group a step
-  float qsum[HD / 32];  // sums of q over each group, in the high parts' columns
+  v8h qsum;             // and of the minima: sums of q over each group
   float mult;      // log2 units of a score's accumulator unit, a power of two
   f4 o[HD / 16];   // rows: heads (high, then low parts), columns: dims 16 e + j
-  f4 om;           // the minima's part, columns: groups
+  f4 om;           // the middles' part, columns: groups, then the sum of the weights
   float ref;       // log2 units of the head's reference score
-  float sum;       // weights of this lane's positions
   int e;           // V steps are below 2^e
   uint32_t bound;  // 2^e as two halves
 };
@@ -541,7 +598,6 @@ static __device__ __forceinline__ void raise(Wave<HD> &s, const float (&v)[8], c
   top = xor32_max(xor16_max(top));  // same in both columns of a head
   const float ref = top - s.ref > kSlack ? top : s.ref, f = exp2f(s.ref - ref);
   s.ref = ref;
-  s.sum *= f;
   // steps that are no NaN, as integers in their order
   int big = 0;
 #pragma unroll
@@ -577,21 +633,20 @@ static __device__ __forceinline__ void scores(const Wave<HD> &s, Pair<HD> &b, in
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    f4 sc = zero;
+    const v8h m = as_v8h(b.km[x][0], NG == 4 ? b.km[x][NG / 2 - 1] : 0u, 0u, 0u);
+    f4 sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(m, s.qsum, zero, 0, 0, 0);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(mid_codes8(b.kc[x][g]), s.q[g], zero, 0, 0, 0);
+      const f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(b.kc[x][g]), s.q[g], zero, 0, 0, 0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float step = half_of(b.ks[x][2 * g + (r >> 1)], r & 1);
-        const float mid = fmaf(8.0f, step, half_of(b.km[x][(r * NG + g) >> 1], g & 1));
-        sc[r] = fmaf(step, acc[r], fmaf(mid, s.qsum[g], sc[r]));
-      }
+      for (int r = 0; r < 4; ++r)
+        sc[r] = fmaf(half_of(b.ks[x][2 * g + (r >> 1)], r & 1), acc[r], sc[r]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[4 * x + r] = sc[r] + row_xor8(sc[r]);  // high and low parts of the query
   }
   if (n < 32) {
+    asm volatile("");  // (a branch, not selects in every pair)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (16 * (i >> 2) + 4 * c + (i & 3) >= n) v[i] = -INFINITY;
@@ -604,8 +659,7 @@ static __device__ __forceinline__ void weigh(Wave<HD> &s, Pair<HD> &b, int n, in
   constexpr int NG = HD / 32, NH = HD / 64;
   const int j = l & 15;
   if (n < 32) cut_values(b, n, l);
-  const float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])),
-                          fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+  const float top = fmaxf(fmaxf(fmaxf(fmaxf(v[0], v[1]), v[2]), fmaxf(fmaxf(v[3], v[4]), v[5])), fmaxf(v[6], v[7]));
   const bool over = max2(max2(max2(b.vo[0][0], b.vo[0][1]), max2(b.vo[1][0], b.vo[1][1])), s.bound) != s.bound;
   if (__any(fmaf(top, s.mult, -s.ref) > kSlack || over)) raise(s, v, b.vo, l);
   const float unit = ldexpf(1.0f, -s.e), low = j < 8 ? 0.0f : 1.0f;
@@ -614,22 +668,31 @@ static __device__ __forceinline__ void weigh(Wave<HD> &s, Pair<HD> &b, int n, in
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     p[i] = __builtin_amdgcn_exp2f(fmaf(v[i], s.mult, shift));
-    s.sum += p[i];
     pu[i] = p[i] * unit;
   }
   auto part = [&](const float (&x)[8]) {
     v8h a;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = half_part(x[i], low);
+    for (int i = 0; i < 8; i += 2) {
+      const v2h h = half_parts(x[i], x[i + 1], low);
+      a[i] = h.x;
+      a[i + 1] = h.y;
+    }
     return a;
   };
   v8h mid, rest;  // the middle of group j's range, code 8, in two parts
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int x = i >> 2, y = (i & 3) >> 1;
-    const float m = fmaf(8.0f, half_of(b.vo[x][y], i & 1), half_of(b.vm[x][y], i & 1));
-    mid[i] = (_Float16)m;
-    rest[i] = (_Float16)(m - (float)mid[i]);
+  for (int i = 0; i < 8; i += 2) {
+    const uint32_t o = b.vo[i >> 2][(i & 3) >> 1], m = b.vm[i >> 2][(i & 3) >> 1];
+    float y = fmaf(8.0f, half_of(o, 0), half_of(m, 0)), z = fmaf(8.0f, half_of(o, 1), half_of(m, 1));
+    asm("" : "+v"(y), "+v"(z));
+    uint32_t h = __builtin_bit_cast(uint32_t, v2h{(_Float16)y, (_Float16)z});
+    asm("" : "+v"(h));
+    const v2h p = __builtin_bit_cast(v2h, h);
+    mid[i] = p.x;
+    mid[i + 1] = p.y;
+    rest[i] = (_Float16)(y - (float)p.x);
+    rest[i + 1] = (_Float16)(z - (float)p.y);
   }
   const v8h pp = part(p);
   s.om = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp, mid, s.om, 0, 0, 0);
@@ -639,17 +702,17 @@ static __device__ __forceinline__ void weigh(Wave<HD> &s, Pair<HD> &b, int n, in
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      x[i] = half_of(b.vs[i >> 2][2 * g + ((i & 3) >> 1)], i & 1) * pu[i];
+      x[i] = fmaf(half_of(b.vs[i >> 2][2 * g + ((i & 3) >> 1)], i & 1), pu[i], 0.0f);
     const v8h a = part(x);
     // blocks 2 g, 2 g + 1: nibbles 2 (g % 2), + 1 of the words of unit g / 2
     const int h = g >> 1, sh = 8 * (g & 1);
     const uint32_t w[4] = {b.vc[0][h] >> sh, b.vc[0][NH + h] >> sh, b.vc[1][h] >> sh,
                            b.vc[1][NH + h] >> sh};
     s.o[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-        a, as_v8h(mid_code<0>(w[0]), mid_code<0>(w[1]), mid_code<0>(w[2]), mid_code<0>(w[3])),
+        a, as_v8h(code_pair<0, true>(w[0]), code_pair<0, true>(w[1]), code_pair<0, true>(w[2]), code_pair<0, true>(w[3])),
         s.o[2 * g], 0, 0, 0);
     s.o[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-        a, as_v8h(mid_code<1>(w[0]), mid_code<1>(w[1]), mid_code<1>(w[2]), mid_code<1>(w[3])),
+        a, as_v8h(code_pair<1, true>(w[0]), code_pair<1, true>(w[1]), code_pair<1, true>(w[2]), code_pair<1, true>(w[3])),
         s.o[2 * g + 1], 0, 0, 0);
   }
 }
@@ -686,21 +749,31 @@ static __device__ __forceinline__ void load_query(Wave<HD> &s, const float *q, i
       v[g][i] = ldexpf(v[g][i], -e);
       sum += v[g][i];
     }
-    sum = xor32_add(xor16_add(sum));
-    s.qsum[g] = j < 8 ? sum * 0x1p-10f : 0.0f;  // (codes come times 2^-10)
-    constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};  // of mid_codes8
+    sum = xor32_add(xor16_add(sum)) * 0x1p-10f;  // (codes come times 2^-10)
+    // high and low parts in the columns, what both leave in a second k-chunk
+    const _Float16 sh = (_Float16)sum, sl = (_Float16)(sum - (float)sh);
+    const float rest = (sum - (float)sh) - (float)sl;
+    s.qsum[g] = (_Float16)(c == 0 ? (j < 8 ? (float)sh : (float)sl) : c == 1 && j < 8 ? rest : 0.0f);
+    constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};  // of codes8
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s.q[g][i] = half_part(v[g][order[i]], low);
+    for (int i = 0; i < 8; i += 2) {
+      const v2h h = half_parts(v[g][order[i]], v[g][order[i + 1]], low);
+      s.q[g][i] = h.x;
+      s.q[g][i + 1] = h.y;
     }
   }
+#pragma unroll
+  for (int g = NG; g < 8; ++g) s.qsum[g] = (_Float16)0.0f;
 }
 
 template <int HD>
 struct DecodeLds {
-  float o[kWaves][kMaxGroup][HD];
+  union {
+    Slot<HD> ring[kWaves][kRing];
+    float o[kWaves][kMaxGroup][HD];
+  };
   float ref[kWaves][kMaxGroup], sum[kWaves][kMaxGroup];
-  int scan[kWaves], item[6];
+  int scan[kWaves], live[kWaves], trial[3][kWaves], item[6];
 };
 
 struct MergeItem {  // of a (lane, KV head): its chunks' records
@@ -712,14 +785,17 @@ static __device__ __forceinline__ int chunk_first(int ch, int pages, int chunks)
   return ch * (pages / chunks) + min(ch, pages % chunks);
 }
 
-// Work items: (lane, KV head, chunk of its pages). Q, the most pages of a
-// chunk, comes from the batch's own lengths: about kTargetItems items share
-// it out, `least` pages each at least. The chunks of a lane are of equal size to a page, so
-// where there are several they hold Q / 2 pages at least.
+// Work items: (lane, KV head, chunk of its pages), a workgroup each. Q, the
+// most pages of a chunk, comes from the batch's own lengths: the smallest of
+// a few that leaves no more items than the device holds workgroups (`slots`),
+// so that they all run at once and end together, `least` pages though. (With
+// more than slots / 2 contexts: 2 U / slots, U the batch's pages.) The chunks
+// of a context are of equal size to a page, so where there are several they
+// hold Q / 2 pages at least.
 template <int HD>
-__global__ __launch_bounds__(64 * kWaves, 2) void kv4_decode_kernel(AttnArgs a, int least,
-                                                                 MergeItem *merge, float *records) {
-  __shared__ DecodeLds<HD> s;
+__global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_kernel(
+    AttnArgs a, int least, int slots, MergeItem *merge, float *records) {
+  __shared__ __align__(16) DecodeLds<HD> s;
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int c = l >> 4, j = l & 15;
   const int Hkv = a.kv.heads, G = a.num_heads / Hkv;
@@ -727,30 +803,61 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_decode_kernel(AttnArgs a, 
 
   // the lanes' pages: a thread holds `per` lanes
   const int per = (a.lanes + 64 * kWaves - 1) / (64 * kWaves);
-  int pages[4], mine = 0;
+  int pages[4], mine = 0, live = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int at = t * per + i;
     const int n = i < per && at < a.lanes ? a.ctx[at] : 0;
     pages[i] = n > 0 && n <= a.max_ctx ? (n + kPage - 1) / kPage : 0;
     mine += pages[i];
+    live += pages[i] > 0;
   }
-  const int pages_in = wave_scan_dpp(mine);
-  if (l == 63) s.scan[w] = pages_in;
+  const int pages_in = wave_scan_dpp(mine), live_in = wave_scan_dpp(live);
+  if (l == 63) {
+    s.scan[w] = pages_in;
+    s.live[w] = live_in;
+  }
   __syncthreads();
-  int total = 0, pages_before = pages_in - mine;
+  int total = 0, pages_before = pages_in - mine, segments = 0;
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) {
     if (i < w) pages_before += s.scan[i];
     total += s.scan[i];
+    segments += s.live[i];
   }
-  __syncthreads();
-  // (even, so that half of it is whole)
-  const int Q = (max(least, (total * Hkv + kTargetItems - 1) / kTargetItems) + 1) & ~1;
+  total *= Hkv;
+  segments *= Hkv;
+  const int room = max(slots - segments, slots / 2);
+  int Q = max(least, (total + room - 1) / room);
+  if (Q > least && segments < slots / 2) {
+    // Q leaves slots items at most; try Q - k / 4 of the way to the mean
+    const int low = max(least, (total + slots - 1) / slots), step = (Q - low + 3) / 4;
+    int n[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const int q = max(low, Q - (k + 1) * step);
+      n[k] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < per) n[k] += (pages[i] + q - 1) / q;
+      n[k] = wave_scan_dpp(n[k] * Hkv);
+      if (l == 63) s.trial[k][w] = n[k];
+    }
+    __syncthreads();
+    const int full = Q;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const int all = s.trial[k][0] + s.trial[k][1] + s.trial[k][2] + s.trial[k][3];
+      if (all <= slots) Q = max(low, full - (k + 1) * step);
+    }
+  }
+  Q = (Q + 1) & ~1;  // so that half of it is whole
   int items = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) items += (pages[i] + Q - 1) / Q * Hkv;
+  for (int i = 0; i < 4; ++i)
+    if (i < per) items += (pages[i] + Q - 1) / Q * Hkv;
   const int items_in = wave_scan_dpp(items);
+  __syncthreads();
   if (l == 63) s.scan[w] = items_in;
   __syncthreads();
   int all = 0, items_before = items_in - items;
@@ -802,11 +909,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_decode_kernel(AttnArgs a, 
   for (int e = 0; e < HD / 16; ++e) s_w.o[e] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   s_w.om = f4{0.0f, 0.0f, 0.0f, 0.0f};
   s_w.ref = kNoRef;
-  s_w.sum = 0.0f;
   s_w.e = -14;
   s_w.bound = 1u << 10 | 1u << 26;
   load_query(s_w, a.q + ((size_t)lane * a.num_heads + h * G) * HD, G, l);
 
+  if (l < kRing * 8) s.ring[w][l >> 3].one[l & 7] = (l & 7) < 4 ? 0 : 0x3C00;
   // a wave takes pairs of pages w, w + kWaves, ... of the chunk
   const int32_t *table = a.table + (size_t)lane * a.max_pages;
   const uint8_t *head_base = a.kv.base + (size_t)(2 * h) * (10 * HD);
@@ -824,21 +931,27 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_decode_kernel(AttnArgs a, 
     auto tile = [&](int i, int x) {
       return head_base + (size_t)(uint32_t)__builtin_amdgcn_readlane((int)id, 2 * i + x) * a.kv.page_bytes;
     };
-    Pair<HD> b;
-    load_keys(b, tile(0, 0), tile(0, 1), l);
-    load_values(b, tile(0, 0), tile(0, 1), l);
+    // (past the last pair it is requested again and not used)
+    auto request = [&](int i) {
+      const int k = min(i, n - 1);
+      copy_pair(&s.ring[w][i % kRing], tile(k, 0), tile(k, 1), l);
+    };
+    for (int i = 0; i < kRing; ++i) request(i);
     for (int i = 0; i < n; ++i) {
-      // the next pair's keys are requested once this one's are used up, and its values
-      // after these; past the last pair they are requested again and not used
-      const int next = min(i + 1, n - 1), left = min(32, stop - (p0 + i * 2 * kWaves) * kPage);
-      const uint8_t *ta = tile(next, 0), *tb = tile(next, 1);
+      const int left = min(32, stop - (p0 + i * 2 * kWaves) * kPage);
+      const Slot<HD> *slot = &s.ring[w][i % kRing];
+      arrive<(kRing - 1) * kPairLoads<HD>>();
+      Pair<HD> b;
       float x[8];
+      read_keys(b, slot, l);
       scores(s_w, b, left, l, x);
-      load_keys(b, ta, tb, l);
+      read_values(b, slot, l);
       weigh(s_w, b, left, l, x);
-      load_values(b, ta, tb, l);
+      request(i + kRing);
     }
   }
+  arrive<0>();
+  __syncthreads();  // the ring's room takes the waves' outputs
 
   // the waves' states, then their sums weighted by 2^(reference - the largest)
   const float unit = ldexpf(1.0f, s_w.e + 10);
@@ -854,11 +967,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_decode_kernel(AttnArgs a, 
       const float v = fmaf(xor32_add(s_w.o[e][r]), unit, m);
       if (c < 2) s.o[w][4 * c + r][16 * e + j] = v;
     }
-  const float sum = xor32_add(xor16_add(s_w.sum));
-  if (l < kMaxGroup) {
-    s.ref[w][l] = s_w.ref;
-    s.sum[w][l] = sum;
-  }
+  if (l < kMaxGroup) s.ref[w][l] = s_w.ref;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (c < 2 && j == HD / 32) s.sum[w][4 * c + r] = om[r];
   bad = __syncthreads_or(bad);
   float *rec = records + (size_t)((start + first) / (Q / 2)) * (kMaxGroup * (HD + 2));
   for (int i = t; i < G * HD; i += 64 * kWaves) {
@@ -987,7 +1099,7 @@ int pool_view(const glacier_hip_kv4_pool_t *p, uint32_t layer, gk::Kv4 *out) {
   return GLACIER_HIP_OK;
 }
 
-size_t kMergeBytes(uint32_t lanes, uint32_t heads) {
+size_t merge_bytes(uint32_t lanes, uint32_t heads) {
   return ((size_t)lanes * heads * sizeof(gk::MergeItem) + 255) & ~(size_t)255;
 }
 
@@ -1025,16 +1137,17 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
     const bool split = (max_ctx + gk::kPage - 1) / gk::kPage > (uint32_t)gk::kWholePages;
     const int least = split ? gk::kSplitPages : gk::kWholePages;
     auto *merge = split ? (gk::MergeItem *)ws : nullptr;
-    float *records = (float *)((char *)ws + kMergeBytes(lanes, pool->num_kv_heads));
-    const uint64_t each = ((max_ctx + gk::kPage - 1) / gk::kPage + least - 1) / least;
-    const uint32_t items = (uint32_t)std::min<uint64_t>(
-        (uint64_t)lanes * a.kv.heads * each, (uint64_t)lanes * a.kv.heads + gk::kTargetItems);
-    const uint32_t grid = std::max(items, lanes);
+    float *records = (float *)((char *)ws + merge_bytes(lanes, pool->num_kv_heads));
+    const int slots = std::min(gk::kMaxSlots, ctx->props.multiProcessorCount * (pool->head_dim == 128 ? 3 : 4));
+    // items at most: slots, or where there are many contexts one each and slots / 2 more
+    const uint64_t heads = (uint64_t)lanes * a.kv.heads, each = ((max_ctx + gk::kPage - 1) / gk::kPage + least - 1) / least;
+    const uint64_t most = heads <= (uint64_t)slots / 2 ? slots : heads + slots / 2;
+    const uint32_t grid = (uint32_t)std::max<uint64_t>(lanes, std::min(heads * each, most));
     if (pool->head_dim == 128) {
-      gk::kv4_decode_kernel<128><<<grid, 64 * gk::kWaves, 0, st>>>(a, least, merge, records);
+      gk::kv4_decode_kernel<128><<<grid, 64 * gk::kWaves, 0, st>>>(a, least, slots, merge, records);
       if (split) gk::kv4_merge_kernel<128><<<lanes * num_heads, 256, 0, st>>>(a, merge, records);
     } else {
-      gk::kv4_decode_kernel<64><<<grid, 64 * gk::kWaves, 0, st>>>(a, least, merge, records);
+      gk::kv4_decode_kernel<64><<<grid, 64 * gk::kWaves, 0, st>>>(a, least, slots, merge, records);
       if (split) gk::kv4_merge_kernel<64><<<lanes * num_heads, 256, 0, st>>>(a, merge, records);
     }
     GH_CHECK(ctx, hipGetLastError());
@@ -1155,7 +1268,7 @@ uint64_t glacier_hip_kv4_attention_workspace_bytes(uint32_t lanes, uint32_t max_
       num_heads % num_kv_heads != 0 || num_heads / num_kv_heads == 0 ||
       num_heads / num_kv_heads > (uint32_t)gk::kMaxGroup)
     return 0;
-  return kMergeBytes(lanes, num_kv_heads) +
+  return merge_bytes(lanes, num_kv_heads) +
          (uint64_t)gk::kMaxRecords * gk::kMaxGroup * (head_dim + 2) * sizeof(float);
 }
 
