@@ -251,92 +251,6 @@ struct AttnArgs {
   float *out;
 };
 
-// One workgroup a (row, KV head): 256 positions at a time, a thread scores
-// each for the G query heads, then every thread adds up its dims.
-template <int HD>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
-  __shared__ float qs[kMaxGroup][HD], sc[kMaxGroup][256], top_s[kMaxGroup], keep_s[kMaxGroup],
-      sum_s[kMaxGroup];
-  const int t = threadIdx.x, r = blockIdx.x, h = blockIdx.y, G = a.num_heads / a.kv.heads;
-  int lane = r, n = 1, first = r;
-  if (a.row_start) {
-    if (r >= a.row_start[a.lanes]) return;
-    int lo = 0, hi = a.lanes - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (a.row_start[mid + 1] > r) hi = mid;
-      else lo = mid + 1;
-    }
-    lane = lo;
-    first = a.row_start[lane];
-    n = a.row_start[lane + 1] - first;
-  }
-  const int ctx = a.ctx[lane];
-  bool bad = ctx < 0 || ctx > a.max_ctx || (a.row_start && n > ctx);
-  const int seen = bad ? 0 : ctx - (first + n - 1 - r) * (a.row_start != nullptr);
-  const float *q = a.q + ((size_t)r * a.num_heads + h * G) * HD;
-  for (int i = t; i < G * HD; i += 256) qs[i / HD][i % HD] = q[i] / sqrtf((float)HD);
-  if (t < kMaxGroup) {
-    top_s[t] = -INFINITY;
-    sum_s[t] = 0.0f;
-  }
-  constexpr int PER = kMaxGroup * HD / 256;
-  float acc[PER] = {};
-  const int32_t *pages = a.table + (size_t)lane * a.max_pages;
-  for (int j0 = 0; j0 < seen; j0 += 256) {
-    __syncthreads();
-    const int j = j0 + t;
-    for (int g = 0; g < G; ++g) sc[g][t] = -INFINITY;
-    if (j < seen) {
-      const uint32_t page = (uint32_t)pages[j / kPage];
-      if (page >= a.kv.page_count) bad = true;
-      else {
-        const uint8_t *tile = tile_of(a.kv, page, h, 0, 10 * HD);
-        float s[kMaxGroup] = {};
-        for (int d = 0; d < HD; ++d) {
-          const float x = kv4_value<HD>(tile, 0, j % kPage, d);
-          for (int g = 0; g < G; ++g) s[g] = fmaf(qs[g][d], x, s[g]);
-        }
-        for (int g = 0; g < G; ++g) sc[g][t] = s[g];
-      }
-    }
-    bad = __syncthreads_or(bad);
-    if (bad) break;
-    if (t < G) {
-      float top = top_s[t], nan = 0.0f;
-      for (int i = 0; i < 256; ++i) {
-        top = fmaxf(top, sc[t][i]);
-        nan += isnan(sc[t][i]) ? 1.0f : 0.0f;
-      }
-      if (nan > 0.0f) top = __uint_as_float(0x7FC00000u);
-      float sum = 0.0f;
-      for (int i = 0; i < 256; ++i) sum += sc[t][i] = expf(sc[t][i] - top);
-      keep_s[t] = top_s[t] == -INFINITY ? 0.0f : expf(top_s[t] - top);
-      sum_s[t] = sum_s[t] * keep_s[t] + sum;
-      top_s[t] = top;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int g = (t + 256 * i) / HD, d = (t + 256 * i) % HD;
-      if (g >= G) continue;
-      float o = acc[i] * keep_s[g];
-      for (int jj = 0; jj < min(256, seen - j0); ++jj) {
-        const uint8_t *tile = tile_of(a.kv, (uint32_t)pages[(j0 + jj) / kPage], h, 1, 10 * HD);
-        o = fmaf(sc[g][jj], kv4_value<HD>(tile, 1, jj % kPage, d), o);
-      }
-      acc[i] = o;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int g = (t + 256 * i) / HD, d = (t + 256 * i) % HD;
-    if (g < G)
-      a.out[((size_t)r * a.num_heads + h * G + g) * HD + d] =
-          bad ? __uint_as_float(0x7FC00000u) : seen == 0 ? 0.0f : acc[i] / sum_s[g];
-  }
-}
-
 // ---------------------------------------------------------------------------
 // Decode attention
 // ---------------------------------------------------------------------------
@@ -719,51 +633,144 @@ static __device__ __forceinline__ void weigh(Wave<HD> &s, Pair<HD> &b, int n, in
 
 // The query operands of one row's heads: q log2(e) / sqrt(HD) = 2^e q', the
 // largest |q'| of a head in [2^13, 2^14), split into fp16 high and low parts.
+// The waves of a workgroup split a group each and share them in LDS.
 template <int HD>
-static __device__ __forceinline__ void load_query(Wave<HD> &s, const float *q, int G, int l) {
+struct QueryLds {
+  v8h q[HD / 32][64];
+  float sum[HD / 32][16];  // of the group, by column
+};
+template <int HD>
+static __device__ __forceinline__ void load_query(Wave<HD> &s, QueryLds<HD> &lds, const float *q, int G,
+                                                  int w, int l) {
   constexpr int NG = HD / 32;
   const int c = l >> 4, j = l & 15, head = j & 7;
   const float unit = 1.44269504088896341f / sqrtf((float)HD);
-  float v[NG][8];
-  float top = 0.0f;
+  float4 v[NG][2];
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     const float *p = q + (size_t)(head < G ? head : 0) * HD + 32 * g + 8 * c;
-    const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
-    const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[g][i] = head < G ? w[i] * unit : 0.0f;
-      top = fmaxf(top, fabsf(v[g][i]));
-    }
+    v[g][0] = *(const float4 *)p;
+    v[g][1] = *(const float4 *)(p + 4);
   }
-  top = xor32_max(xor16_max(top));
-  const int e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+  float top = 0.0f;
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      top = fmaxf(fmaxf(fmaxf(fmaxf(top, fabsf(v[g][i].x)), fabsf(v[g][i].y)), fabsf(v[g][i].z)), fabsf(v[g][i].w));
+  top = xor32_max(xor16_max(top)) * unit;
+  // (a query below 2^-106 stays below 2^13)
+  const int e = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0, -120);
   s.mult = ldexpf(1.0f, e + 10);
-  const float low = j < 8 ? 0.0f : 1.0f;
+  const float scale = head < G ? ldexpf(1.0f, -e) : 0.0f, low = j < 8 ? 0.0f : 1.0f;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    float sum = 0.0f;
+    if (w % NG != g) continue;
+    const float x[8] = {v[g][0].x, v[g][0].y, v[g][0].z, v[g][0].w, v[g][1].x, v[g][1].y, v[g][1].z, v[g][1].w};
+    float y[8], sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[g][i] = ldexpf(v[g][i], -e);
-      sum += v[g][i];
+      y[i] = x[i] * unit * scale;
+      sum += y[i];
     }
     sum = xor32_add(xor16_add(sum)) * 0x1p-10f;  // (codes come times 2^-10)
+    constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};  // of codes8
+    v8h o;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const v2h h = half_parts(y[order[i]], y[order[i + 1]], low);
+      o[i] = h.x;
+      o[i + 1] = h.y;
+    }
+    if (w < NG) {
+      lds.q[g][l] = o;
+      if (l < 16) lds.sum[g][l] = sum;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    s.q[g] = lds.q[g][l];
+    const float sum = lds.sum[g][j];
     // high and low parts in the columns, what both leave in a second k-chunk
     const _Float16 sh = (_Float16)sum, sl = (_Float16)(sum - (float)sh);
     const float rest = (sum - (float)sh) - (float)sl;
     s.qsum[g] = (_Float16)(c == 0 ? (j < 8 ? (float)sh : (float)sl) : c == 1 && j < 8 ? rest : 0.0f);
-    constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};  // of codes8
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const v2h h = half_parts(v[g][order[i]], v[g][order[i + 1]], low);
-      s.q[g][i] = h.x;
-      s.q[g][i + 1] = h.y;
-    }
   }
 #pragma unroll
   for (int g = NG; g < 8; ++g) s.qsum[g] = (_Float16)0.0f;
+}
+
+struct WorkItem {
+  int lane, head, ctx, chunk, chunks, start, most;  // lane < 0: none
+};
+
+// n / d rounded up, n < 2^24.
+static __device__ __forceinline__ int ceil_div(int n, int d, float rd) {
+  int q = (int)((float)n * rd);
+  q += q * d < n;
+  q -= (q - 1) * d >= n;
+  return q;
+}
+
+// Item blockIdx.x of the list, by one wave (l its thread): a thread holds
+// a.lanes / 64 lanes.
+static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int least, int slots, int l) {
+  const int per = (a.lanes + 63) / 64, Hkv = a.kv.heads;
+  auto pages_of = [&](int i) {
+    const int at = l * per + i, n = at < a.lanes ? a.ctx[at] : 0;
+    return n > 0 && n <= a.max_ctx ? (n + kPage - 1) / kPage : 0;
+  };
+  const int only = pages_of(0);
+  int mine = only, live = only > 0;
+  for (int i = 1; i < per; ++i) {
+    const int p = pages_of(i);
+    mine += p;
+    live += p > 0;
+  }
+  const int pages_in = wave_scan_dpp(mine);
+  const int total = __builtin_amdgcn_readlane(pages_in, 63) * Hkv;
+  const int segments = __builtin_amdgcn_readlane(wave_scan_dpp(live), 63) * Hkv;
+  auto chunks_of = [&](int q) {  // of the thread's lanes
+    const float r = 1.0f / (float)q;
+    int n = ceil_div(only, q, r);
+    for (int i = 1; i < per; ++i) n += ceil_div(pages_of(i), q, r);
+    return n;
+  };
+  const int room = max(slots - segments, slots / 2);
+  int Q = max(least, (total + room - 1) / room);
+  if (Q > least && segments < slots / 2) {
+    // Q leaves slots items at most; try k / 4 of the way down to the mean
+    const int full = Q, low = max(least, (total + slots - 1) / slots), step = (Q - low + 3) / 4;
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+      const int q = max(low, full - k * step);
+      if (__builtin_amdgcn_readlane(wave_scan_dpp(chunks_of(q)), 63) * Hkv <= slots) Q = q;
+    }
+  }
+  Q = (Q + 1) & ~1;  // so that half of it is whole
+  const int count = chunks_of(Q) * Hkv, last = wave_scan_dpp(count);
+  const int item = blockIdx.x;
+  WorkItem m{-1, 0, 0, 0, 0, 0, Q};
+  const uint64_t past = __ballot(last > item);
+  if (past == 0) return m;
+  const int owner = __builtin_ctzll(past);
+  // the owner's lanes, by every thread alike
+  int at = __builtin_amdgcn_readlane(last - count, owner), pb = __builtin_amdgcn_readlane(pages_in - mine, owner);
+  const float r = 1.0f / (float)Q;
+  for (int i = 0; i < per; ++i) {
+    const int lane = owner * per + i, n = lane < a.lanes ? a.ctx[lane] : 0;
+    const int p = n > 0 && n <= a.max_ctx ? (n + kPage - 1) / kPage : 0;
+    const int chunks = ceil_div(p, Q, r), k = item - at;
+    if (k < chunks * Hkv) {
+      const int head = k / chunks;
+      m = {lane, head, n, k - head * chunks, chunks, pb * Hkv + head * p, Q};
+      break;
+    }
+    at += chunks * Hkv;
+    pb += p;
+  }
+  return m;
 }
 
 template <int HD>
@@ -772,8 +779,9 @@ struct DecodeLds {
     Slot<HD> ring[kWaves][kRing];
     float o[kWaves][kMaxGroup][HD];
   };
-  float ref[kWaves][kMaxGroup], sum[kWaves][kMaxGroup];
-  int scan[kWaves], live[kWaves], trial[3][kWaves], item[6];
+  float ref[kWaves][kMaxGroup], sum[kWaves][kMaxGroup], f[kWaves][kMaxGroup];
+  QueryLds<HD> query;
+  WorkItem item;
 };
 
 struct MergeItem {  // of a (lane, KV head): its chunks' records
@@ -801,72 +809,6 @@ __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_ker
   const int Hkv = a.kv.heads, G = a.num_heads / Hkv;
   const float nan = __uint_as_float(0x7FC00000u);
 
-  // the lanes' pages: a thread holds `per` lanes
-  const int per = (a.lanes + 64 * kWaves - 1) / (64 * kWaves);
-  int pages[4], mine = 0, live = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int at = t * per + i;
-    const int n = i < per && at < a.lanes ? a.ctx[at] : 0;
-    pages[i] = n > 0 && n <= a.max_ctx ? (n + kPage - 1) / kPage : 0;
-    mine += pages[i];
-    live += pages[i] > 0;
-  }
-  const int pages_in = wave_scan_dpp(mine), live_in = wave_scan_dpp(live);
-  if (l == 63) {
-    s.scan[w] = pages_in;
-    s.live[w] = live_in;
-  }
-  __syncthreads();
-  int total = 0, pages_before = pages_in - mine, segments = 0;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    if (i < w) pages_before += s.scan[i];
-    total += s.scan[i];
-    segments += s.live[i];
-  }
-  total *= Hkv;
-  segments *= Hkv;
-  const int room = max(slots - segments, slots / 2);
-  int Q = max(least, (total + room - 1) / room);
-  if (Q > least && segments < slots / 2) {
-    // Q leaves slots items at most; try Q - k / 4 of the way to the mean
-    const int low = max(least, (total + slots - 1) / slots), step = (Q - low + 3) / 4;
-    int n[3];
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const int q = max(low, Q - (k + 1) * step);
-      n[k] = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < per) n[k] += (pages[i] + q - 1) / q;
-      n[k] = wave_scan_dpp(n[k] * Hkv);
-      if (l == 63) s.trial[k][w] = n[k];
-    }
-    __syncthreads();
-    const int full = Q;
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const int all = s.trial[k][0] + s.trial[k][1] + s.trial[k][2] + s.trial[k][3];
-      if (all <= slots) Q = max(low, full - (k + 1) * step);
-    }
-  }
-  Q = (Q + 1) & ~1;  // so that half of it is whole
-  int items = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < per) items += (pages[i] + Q - 1) / Q * Hkv;
-  const int items_in = wave_scan_dpp(items);
-  __syncthreads();
-  if (l == 63) s.scan[w] = items_in;
-  __syncthreads();
-  int all = 0, items_before = items_in - items;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    if (i < w) items_before += s.scan[i];
-    all += s.scan[i];
-  }
-
   // a lane without positions, or with a length that does not hold
   if ((int)blockIdx.x < a.lanes) {
     const int n = a.ctx[blockIdx.x];
@@ -877,31 +819,18 @@ __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_ker
         for (int i = t; i < Hkv; i += 64 * kWaves) merge[blockIdx.x * Hkv + i].chunks = 0;
     }
   }
-  const int item = blockIdx.x;
-  if (item >= all) return;
-  if (item >= items_before && item < items_before + items) {
-    int at = items_before, pb = pages_before;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int chunks = (pages[i] + Q - 1) / Q, r = item - at;
-      if (r >= 0 && r < chunks * Hkv) {
-        s.item[0] = t * per + i;
-        s.item[1] = r / chunks;
-        s.item[2] = r % chunks;
-        s.item[3] = chunks;
-        s.item[4] = pages[i];
-        s.item[5] = pb * Hkv + r / chunks * pages[i];
-      }
-      at += chunks * Hkv;
-      pb += pages[i];
-    }
+  if (w == 0) {
+    const WorkItem m = find_item(a, least, slots, l);
+    if (l == 0) s.item = m;
   }
   __syncthreads();
-  const int lane = __builtin_amdgcn_readfirstlane(s.item[0]), h = __builtin_amdgcn_readfirstlane(s.item[1]);
-  const int ch = __builtin_amdgcn_readfirstlane(s.item[2]), chunks = __builtin_amdgcn_readfirstlane(s.item[3]);
-  const int lane_pages = __builtin_amdgcn_readfirstlane(s.item[4]), start = __builtin_amdgcn_readfirstlane(s.item[5]);
+  const int lane = __builtin_amdgcn_readfirstlane(s.item.lane);
+  if (lane < 0) return;
+  const int h = __builtin_amdgcn_readfirstlane(s.item.head), ctx = __builtin_amdgcn_readfirstlane(s.item.ctx);
+  const int ch = __builtin_amdgcn_readfirstlane(s.item.chunk), chunks = __builtin_amdgcn_readfirstlane(s.item.chunks);
+  const int start = __builtin_amdgcn_readfirstlane(s.item.start), Q = __builtin_amdgcn_readfirstlane(s.item.most);
+  const int lane_pages = (ctx + kPage - 1) / kPage;
   const int first = chunk_first(ch, lane_pages, chunks), end = chunk_first(ch + 1, lane_pages, chunks);
-  const int ctx = __builtin_amdgcn_readfirstlane(a.ctx[lane]);
   if (merge && ch == 0 && t == 0) merge[lane * Hkv + h] = {start, lane_pages, chunks, Q / 2};
 
   Wave<HD> s_w;
@@ -911,7 +840,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_ker
   s_w.ref = kNoRef;
   s_w.e = -14;
   s_w.bound = 1u << 10 | 1u << 26;
-  load_query(s_w, a.q + ((size_t)lane * a.num_heads + h * G) * HD, G, l);
+  load_query(s_w, s.query, a.q + ((size_t)lane * a.num_heads + h * G) * HD, G, w, l);
 
   if (l < kRing * 8) s.ring[w][l >> 3].one[l & 7] = (l & 7) < 4 ? 0 : 0x3C00;
   // a wave takes pairs of pages w, w + kWaves, ... of the chunk
@@ -953,45 +882,58 @@ __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_ker
   arrive<0>();
   __syncthreads();  // the ring's room takes the waves' outputs
 
-  // the waves' states, then their sums weighted by 2^(reference - the largest)
+  // the waves' states, then their sums weighted by 2^(reference - the
+  // largest). High and low parts are rows 4 c + r and 8 more, 32 lanes apart:
+  // a swap of blocks e and e + HD / 32 leaves both parts of e in the lower
+  // lanes, of the other in the upper ones.
   const float unit = ldexpf(1.0f, s_w.e + 10);
   float om[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) om[r] = xor32_add(s_w.om[r]);
 #pragma unroll
-  for (int e = 0; e < HD / 16; ++e)
+  for (int e = 0; e < HD / 32; ++e)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float m = e / 2 == 0 ? row_lane<0>(om[r]) : e / 2 == 1 ? row_lane<1>(om[r])
-                      : e / 2 == 2 ? row_lane<2>(om[r]) : row_lane<3>(om[r]);
-      const float v = fmaf(xor32_add(s_w.o[e][r]), unit, m);
-      if (c < 2) s.o[w][4 * c + r][16 * e + j] = v;
+      const v2u x = __builtin_amdgcn_permlane32_swap(__float_as_uint(s_w.o[e][r]),
+                                                     __float_as_uint(s_w.o[e + HD / 32][r]), false, false);
+      const float m = l < 32 ? (e / 2 == 0 ? row_lane<0>(om[r]) : row_lane<1>(om[r]))
+                      : HD == 64 ? row_lane<1>(om[r])
+                                 : (e / 2 == 0 ? row_lane<2>(om[r]) : row_lane<3>(om[r]));
+      s.o[w][4 * (c & 1) + r][16 * e + (l < 32 ? 0 : HD / 2) + j] =
+          fmaf(__uint_as_float(x.x) + __uint_as_float(x.y), unit, m);
     }
   if (l < kMaxGroup) s.ref[w][l] = s_w.ref;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (c < 2 && j == HD / 32) s.sum[w][4 * c + r] = om[r];
   bad = __syncthreads_or(bad);
+  if (t < kMaxGroup) {
+    float top = s.ref[0][t], L = 0.0f;
+#pragma unroll
+    for (int v = 1; v < kWaves; ++v) top = fmaxf(top, s.ref[v][t]);
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float f = __builtin_amdgcn_exp2f(s.ref[v][t] - top);
+      s.f[v][t] = f;
+      L = fmaf(s.sum[v][t], f, L);
+    }
+    s.ref[0][t] = top;
+    s.sum[0][t] = bad ? nan : L;
+  }
+  __syncthreads();
   float *rec = records + (size_t)((start + first) / (Q / 2)) * (kMaxGroup * (HD + 2));
   for (int i = t; i < G * HD; i += 64 * kWaves) {
     const int g = i / HD, d = i % HD;
-    float top = s.ref[0][g];
+    const float L = s.sum[0][g];
+    float O = 0.0f;
 #pragma unroll
-    for (int v = 1; v < kWaves; ++v) top = fmaxf(top, s.ref[v][g]);
-    float L = 0.0f, O = 0.0f;
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
-      const float f = __builtin_amdgcn_exp2f(s.ref[v][g] - top);
-      L = fmaf(s.sum[v][g], f, L);
-      O = fmaf(s.o[v][g][d], f, O);
-    }
-    if (bad) L = nan;
+    for (int v = 0; v < kWaves; ++v) O = fmaf(s.o[v][g][d], s.f[v][g], O);
     if (chunks == 1) {
       a.out[((size_t)lane * a.num_heads + h * G + g) * HD + d] = O / L;
     } else {
       rec[g * (HD + 2) + 2 + d] = O;
       if (d == 0) {
-        rec[g * (HD + 2)] = top;
+        rec[g * (HD + 2)] = s.ref[0][g];
         rec[g * (HD + 2) + 1] = L;
       }
     }
@@ -1055,6 +997,497 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, const MergeI
   }
 }
 
+// ---------------------------------------------------------------------------
+// Attention of row runs
+// ---------------------------------------------------------------------------
+// Columns are (row, query head of the KV head), a row's heads together, so a
+// run of any length and any group size fills tiles of 32 columns a wave, 128
+// a workgroup (a tile). The workgroup walks the keys 32 at a time: two pages'
+// codes become values in LDS once for all columns, each as an fp16 high and
+// low part (a value keeps 22 bits; the codes' steps do not fit the operands
+// as they do with one row a head, whose weights take them), double buffered,
+// a barrier a stage:
+//   scores  S^T = K . Q^T on v_mfma_f32_32x32x16_f16, high.high + high.low +
+//           low.high; lane (h, col) ends with keys 8 (i / 4) + 4 h + i % 4
+//           of its own column in register i,
+//   softmax in registers, a column's reference in its two lanes; it follows
+//           the scores only when one passes it by kSlack, so a stage takes
+//           no cross-lane step,
+//   output  O^T += V^T . P^T: the B operand is the lane's own registers (V's
+//           keys are laid out in their order), so rescaling is lane-local.
+// Long contexts of few columns are cut into chunks of stages (records, merged
+// below) so that they spread over the device.
+typedef float f16v __attribute__((ext_vector_type(16)));
+constexpr int kTile = 128;        // columns of a workgroup
+constexpr int kStage = 32;        // keys of a stage
+constexpr int kMinStages = 8;     // stages of a chunk at least
+constexpr int kRowsSlots = 512;   // workgroups that a batch is cut for, at most
+// A cut tile's longest is over Q = 3 means of a slot, and its lane's tiles
+// average half of it: fewer than slots / 1.5 are cut, into 4 / 3 slots chunks.
+constexpr int kRowsCut = kRowsSlots * 2 / 3 + 8, kRowsRecords = kRowsSlots * 4 / 3 + 16;
+constexpr size_t kRowsHeader = 16384;  // workspace: the cut tiles' count and places, then records
+
+template <int HD>
+struct RowsLds {
+  // [step][high, low][lane] operands of K, [32 dims][16 keys][high, low][lane] of V
+  uint8_t k[2][HD / 16][2][1024], v[2][HD / 32][2][2][1024];
+  // keys whose V group is no number, by group, and whether there are any: of
+  // the stage in use, the next, and one to clear
+  uint32_t odd[3][HD / 32 + 1];
+  int item[8];
+};
+
+struct RowsItem {
+  int lane, head, tile, chunk, chunks, record, split;  // lane < 0: none
+};
+struct RowsTile {  // a cut tile, for the merge
+  int row, head, cols, chunks, record;
+};
+
+static __device__ __forceinline__ float wave_scan_f(float v) {
+  auto d = [](float x, auto f) { return x + __int_as_float(f(__float_as_int(x))); };
+  v = d(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true); });
+  v = d(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true); });
+  v = d(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true); });
+  v = d(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true); });
+  v = d(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false); });
+  return d(v, [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false); });
+}
+
+// Rows of a lane (first, count; none where the run does not lie in the rows).
+static __device__ __forceinline__ void run_of(const AttnArgs &a, int lane, int &first, int &n) {
+  first = lane < a.lanes ? a.row_start[lane] : 0;
+  const int end = lane < a.lanes ? a.row_start[lane + 1] : 0;
+  n = first >= 0 && end <= a.max_rows ? max(0, end - first) : 0;
+}
+
+// Work items: (lane, tile, KV head, chunk), the tiles of a lane from its last
+// on (the longest), by one wave; a thread holds lanes / 64 lanes. A lane's
+// tiles are cut into as many chunks as its longest has shares Q of the
+// batch's stages, a share three times the mean of a slot (tiles of a prompt
+// average half their longest: a prompt that fills the device stays whole).
+// The list is dealt in runs of 256 (a CU each), every other one backwards, so
+// that CUs pair long items with short ones.
+static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int slots, bool split, int l,
+                                                          int *cut_tiles) {
+  const int per = (a.lanes + 63) / 64, Hkv = a.kv.heads, G = a.num_heads / Hkv;
+  auto tiles_of = [&](int i, int &stages) {
+    int first, n;
+    run_of(a, l * per + i, first, n);
+    const int ctx = n > 0 ? a.ctx[l * per + i] : 0;
+    stages = ctx >= n && ctx <= a.max_ctx ? (ctx + kStage - 1) / kStage : 0;
+    return (n * G + kTile - 1) / kTile;
+  };
+  float work = 0.0f;
+  for (int i = 0; i < per; ++i) {
+    int st, first, n;
+    const int tiles = tiles_of(i, st);
+    run_of(a, l * per + i, first, n);
+    work += (float)tiles * ((float)st - 0.5f * (float)n / kStage);
+  }
+  const float total = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_scan_f(work)), 63)) * (float)Hkv;
+  const int Q = split ? max(kMinStages, (int)(3.0f * total / (float)slots) + 1) : 1 << 30;
+  int count = 0, cut = 0, cut_items = 0;
+  for (int i = 0; i < per; ++i) {
+    int st;
+    const int tiles = tiles_of(i, st), chunks = max(1, (st + Q - 1) / Q);
+    count += tiles * Hkv * chunks;
+    if (chunks > 1) {
+      cut += tiles * Hkv;
+      cut_items += tiles * Hkv * chunks;
+    }
+  }
+  const int last = wave_scan_dpp(count), cut_last = wave_scan_dpp(cut), rec_last = wave_scan_dpp(cut_items);
+  const int all = __builtin_amdgcn_readlane(last, 63);
+  *cut_tiles = __builtin_amdgcn_readlane(cut_last, 63);
+  RowsItem m{-1, 0, 0, 0, 0, 0, 0};
+  int item = blockIdx.x;
+  if (item >= all) return m;
+  const int run = item & ~255;
+  if (item & 256) item = run + min(256, all - run) - 1 - (item - run);
+  const int owner = __builtin_ctzll(__ballot(last > item));
+  int at = __builtin_amdgcn_readlane(last - count, owner), tile_at = __builtin_amdgcn_readlane(cut_last - cut, owner);
+  int rec_at = __builtin_amdgcn_readlane(rec_last - cut_items, owner);
+  for (int i = 0; i < per; ++i) {
+    const int lane = owner * per + i;
+    int first, n;
+    run_of(a, lane, first, n);
+    const int ctx = n > 0 ? a.ctx[lane] : 0;
+    const int st = ctx >= n && ctx <= a.max_ctx ? (ctx + kStage - 1) / kStage : 0;
+    const int tiles = (n * G + kTile - 1) / kTile, chunks = max(1, (st + Q - 1) / Q), k = item - at;
+    const int here = tiles * Hkv * chunks;
+    if (k < here) {
+      const int u = k / chunks;
+      m = {lane, u % Hkv, tiles - 1 - u / Hkv, k - u * chunks, chunks, rec_at + k, tile_at + u};
+      break;
+    }
+    at += here;
+    if (chunks > 1) {
+      tile_at += tiles * Hkv;
+      rec_at += here;
+    }
+  }
+  return m;
+}
+
+// What a thread requests of a stage: waves 0 and 1 K codes of a (page,
+// position, chunk c of 8 dims a group), waves 2 and 3 V codes of a (page, four
+// positions c, column j).
+template <int HD>
+struct Raw {
+  uint32_t code[HD / 32];
+  uint32_t step[HD / 16], low[HD / 16];
+};
+
+template <int HD>
+static __device__ __forceinline__ void load_raw(Raw<HD> &r, const uint8_t *tile, int w, int l) {
+  constexpr int NG = HD / 32;
+  const int c = l >> 4, j = l & 15;
+  if (w < 2) {
+    load_words(r.code, tile + j * (HD / 2) + c * (4 * NG));
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+      r.step[g] = *(const uint16_t *)(tile + 8 * HD + 2 * ((j >> 2) * (4 * NG) + g * 4 + (j & 3)));
+    const uint8_t *p = tile + 9 * HD + j * (2 * NG);
+#pragma unroll
+    for (int g = 0; g < NG; g += 2) r.low[g / 2] = *(const uint32_t *)(p + 2 * g);
+  } else {
+    load_words(r.code, tile + (c * 16 + j) * (4 * NG));
+    load_words(r.step, tile + 8 * HD + c * (8 * NG));
+    load_words(r.low, tile + 9 * HD + c * (8 * NG));
+  }
+}
+
+// fp16 high and low parts of two values: the high one truncated, so that the
+// rest is what a mask leaves, that one rounded.
+static __device__ __forceinline__ void two_parts(float x, float y, uint32_t &high, uint32_t &low) {
+  const float rx = x - __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
+  const float ry = y - __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);
+  high = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+  low = __builtin_bit_cast(uint32_t, v2h{(_Float16)rx, (_Float16)ry});
+}
+
+// Stage st from the raw codes; keys: the stage's keys inside the context.
+template <int HD>
+static __device__ __forceinline__ void write_stage(RowsLds<HD> &s, int st, const Raw<HD> &r, int w, int l,
+                                                   int keys, bool bad) {
+  constexpr int NG = HD / 32;
+  const int c = l >> 4, j = l & 15, page = w & 1, buf = st & 1;
+  if (w < 2) {
+    const int key = 16 * page + j;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float step = bad ? __uint_as_float(0x7FC00000u) : half_of(r.step[g], 0);
+      const float low = half_of(r.low[g >> 1], g & 1);
+      const uint32_t even = r.code[g] & 0x0F0F0F0Fu, odd = r.code[g] >> 4 & 0x0F0F0F0Fu;
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        two_parts(fmaf((float)(even >> 8 * i & 0xFFu), step, low), fmaf((float)(odd >> 8 * i & 0xFFu), step, low),
+                  hi[i], lo[i]);
+      const int at = (32 * (c & 1) + key) * 16;
+      *(uint4 *)(s.k[buf][2 * g + (c >> 1)][0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *(uint4 *)(s.k[buf][2 * g + (c >> 1)][1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    return;
+  }
+  const int left = keys - 16 * page - 4 * c;  // of the thread's four positions
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 2 * NG; ++i) most = max2(most, max2(r.step[i] & 0x7FFF7FFFu, r.low[i] & 0x7FFF7FFFu));
+  const bool odd = bad || left < 4 || (most & 0xFFFFu) >= 0x7C00u || most >> 16 >= 0x7C00u;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    float step[4], low[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      step[p] = half_of(r.step[2 * g + (p >> 1)], p & 1);
+      low[p] = half_of(r.low[2 * g + (p >> 1)], p & 1);
+    }
+    if (__any(odd)) {
+      // positions past the context, of no page, or with no number: zeros, the last noted
+      asm volatile("");
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const bool none = bad || p >= left, nan = !(fabsf(step[p]) <= 65504.0f && fabsf(low[p]) <= 65504.0f);
+        if (none || nan) step[p] = low[p] = 0.0f;
+        if (nan && !none && j == 0) {
+          atomicOr(&s.odd[st % 3][g], 1u << (16 * page + 4 * c + p));
+          atomicOr(&s.odd[st % 3][NG], 1u);
+        }
+      }
+    }
+    // blocks 2 g, 2 g + 1: byte g % 2 of unit g / 2 of each position
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float x[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const uint32_t word = r.code[(p >> 1) * (HD / 64) + (g >> 1)];
+        x[p] = fmaf((float)(word >> (16 * (p & 1) + 8 * (g & 1) + 4 * b) & 15u), step[p], low[p]);
+      }
+      uint32_t hi[2], lo[2];
+      two_parts(x[0], x[1], hi[0], lo[0]);
+      two_parts(x[2], x[3], hi[1], lo[1]);
+      const int at = (32 * (c & 1) + 16 * b + j) * 16 + (c >> 1) * 8;
+      *(uint2 *)(s.v[buf][g][page][0] + at) = make_uint2(hi[0], hi[1]);
+      *(uint2 *)(s.v[buf][g][page][1] + at) = make_uint2(lo[0], lo[1]);
+    }
+  }
+}
+
+template <int HD>
+__global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots, int split, int *header,
+                                                       RowsTile *tiles, float *records) {
+  constexpr int S = HD / 16, NG = HD / 32;
+  __shared__ __align__(16) RowsLds<HD> s;
+  const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int Hkv = a.kv.heads, G = a.num_heads / Hkv;
+  const float nan = __uint_as_float(0x7FC00000u);
+  if (w == 0) {
+    int cut;
+    const RowsItem m = find_rows_item(a, slots, split, l, &cut);
+    if (l == 0) {
+      s.item[0] = m.lane;
+      s.item[1] = m.head;
+      s.item[2] = m.tile;
+      s.item[3] = m.chunk;
+      s.item[4] = m.chunks;
+      s.item[5] = m.record;
+      s.item[6] = m.split;
+      if (blockIdx.x == 0 && split) header[0] = cut;
+    }
+  }
+  if (t < 3 * (NG + 1)) s.odd[t / (NG + 1)][t % (NG + 1)] = 0;
+  __syncthreads();
+  const int lane = __builtin_amdgcn_readfirstlane(s.item[0]);
+  if (lane < 0) return;
+  const int h = __builtin_amdgcn_readfirstlane(s.item[1]), tile = __builtin_amdgcn_readfirstlane(s.item[2]);
+  const int chunk = __builtin_amdgcn_readfirstlane(s.item[3]), chunks = __builtin_amdgcn_readfirstlane(s.item[4]);
+  const int record = __builtin_amdgcn_readfirstlane(s.item[5]);
+  int first, n;
+  run_of(a, lane, first, n);
+  first = __builtin_amdgcn_readfirstlane(first);
+  n = __builtin_amdgcn_readfirstlane(n);
+  const int ctx = __builtin_amdgcn_readfirstlane(a.ctx[lane]);
+  const bool valid = ctx >= n && ctx <= a.max_ctx;
+  const int half = l >> 5, cols = n * G;
+  // this lane's column; past the run, the last one again (its output is not written)
+  const int col = kTile * tile + 32 * w + (l & 31), colc = min(col, cols - 1);
+  const int row = colc / G, head = h * G + colc - row * G;
+  const int seen = ctx - n + row + 1;
+  // the tile's stages, and this chunk's
+  const int tile_row = (min(kTile * (tile + 1), cols) - 1) / G;
+  const int all = valid ? (ctx - n + tile_row + 1 + kStage - 1) / kStage : 0;
+  const int s0 = chunk_first(chunk, all, chunks), s1 = chunk_first(chunk + 1, all, chunks);
+  if (split && chunks > 1 && chunk == 0 && t == 0)
+    tiles[s.item[6]] = {first + kTile * tile / G, h, kTile * tile, chunks, record};
+
+  // queries: q log2(e) / sqrt(HD) = 2^e q', the largest |q'| of a column in
+  // [2^13, 2^14), as the B operand in two fp16 parts
+  v8h qh[S], ql[S];
+  float mult;
+  {
+    const float *q = a.q + ((size_t)(first + row) * a.num_heads + head) * HD + 8 * half;
+    const float unit = 1.44269504088896341f / sqrtf((float)HD);
+    float4 v[S][2];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      v[i][0] = *(const float4 *)(q + 16 * i);
+      v[i][1] = *(const float4 *)(q + 16 * i + 4);
+    }
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        top = fmaxf(fmaxf(fmaxf(fmaxf(top, fabsf(v[i][k].x)), fabsf(v[i][k].y)), fabsf(v[i][k].z)), fabsf(v[i][k].w));
+    top = xor32_max(top) * unit;
+    const int e = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0, -120);
+    mult = ldexpf(1.0f, e);
+    const float scale = ldexpf(1.0f, -e);
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const float x[8] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w, v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w};
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) two_parts(x[2 * k] * unit * scale, x[2 * k + 1] * unit * scale, hi[k], lo[k]);
+      qh[i] = as_v8h(hi[0], hi[1], hi[2], hi[3]);
+      ql[i] = as_v8h(lo[0], lo[1], lo[2], lo[3]);
+    }
+  }
+  f16v o[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[g][i] = 0.0f;
+  float ref = kNoRef, sum = 0.0f;
+  int odd = 0;  // groups of this column with no number
+  const bool wave_in = kTile * tile + 32 * w < cols;
+  const int wave_first = __builtin_amdgcn_readfirstlane(seen);  // the fewest and most keys of the wave's columns
+  const int wave_last = __builtin_amdgcn_readlane(seen, 31);
+
+  const int32_t *table = a.table + (size_t)lane * a.max_pages;
+  const int pages = (ctx + kPage - 1) / kPage;
+  const size_t mine = (size_t)(2 * h + (w >> 1)) * (10 * HD);
+  int id_base = -64;
+  uint32_t ids = 0;
+  bool bad = false;
+  Raw<HD> raw;
+  auto request = [&](int st) {  // this wave's page of a stage
+    const int p = 2 * st + (w & 1);
+    if (2 * st >= id_base + 64) {
+      id_base = 2 * st;
+      ids = (uint32_t)table[min(id_base + l, pages - 1)];
+    }
+    const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)ids, min(p, pages - 1) - id_base);
+    bad = id >= a.kv.page_count;
+    load_raw(raw, a.kv.base + (size_t)(bad ? 0 : id) * a.kv.page_bytes + mine, w, l);
+  };
+  if (s0 < s1) {
+    request(s0);
+    write_stage(s, s0, raw, w, l, ctx - s0 * kStage, bad);
+    request(min(s0 + 1, s1 - 1));
+  }
+  __syncthreads();
+  for (int st = s0; st < s1; ++st) {
+    const int buf = st & 1, key0 = st * kStage;
+    if (wave_in && key0 < wave_last) {
+      f16v sc;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        const v8h kh = *(const v8h *)(s.k[buf][i][0] + l * 16), kl = *(const v8h *)(s.k[buf][i][1] + l * 16);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[i], sc, 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[i], sc, 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[i], sc, 0, 0, 0);
+      }
+      if (key0 + kStage > wave_first) {
+        asm volatile("");
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (key0 + 8 * (i >> 2) + 4 * half + (i & 3) >= seen) sc[i] = -INFINITY;
+      }
+      float top = sc[0];
+#pragma unroll
+      for (int i = 1; i < 15; i += 2) top = fmaxf(fmaxf(top, sc[i]), sc[i + 1]);
+      top = fmaxf(top, sc[15]);
+      if (__any(fmaf(top, mult, -ref) > kSlack)) {
+        asm volatile("");
+        const float high = xor32_max(top) * mult;
+        const float next = high - ref > kSlack ? high : ref, f = exp2f(ref - next);
+        ref = next;
+        sum *= f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) o[g] *= f;
+      }
+      const float shift = kShift - ref;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], mult, shift));
+        sum += sc[i];
+      }
+      uint32_t ph[8], pl[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) two_parts(sc[2 * i], sc[2 * i + 1], ph[i], pl[i]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const v8h bh = as_v8h(ph[4 * x], ph[4 * x + 1], ph[4 * x + 2], ph[4 * x + 3]);
+        const v8h bl = as_v8h(pl[4 * x], pl[4 * x + 1], pl[4 * x + 2], pl[4 * x + 3]);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const v8h vh = *(const v8h *)(s.v[buf][g][x][0] + l * 16), vl = *(const v8h *)(s.v[buf][g][x][1] + l * 16);
+          o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, bl, o[g], 0, 0, 0);
+          o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, bh, o[g], 0, 0, 0);
+          o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, bh, o[g], 0, 0, 0);
+        }
+      }
+      if (__builtin_amdgcn_readfirstlane(s.odd[st % 3][NG])) {
+        const int k = min(kStage, seen - key0);
+        const uint32_t shown = k <= 0 ? 0u : k >= 32 ? 0xFFFFFFFFu : (1u << k) - 1;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) odd |= (s.odd[st % 3][g] & shown) != 0 ? 1 << g : 0;
+      }
+    }
+    if (st + 1 < s1) {
+      write_stage(s, st + 1, raw, w, l, ctx - (st + 1) * kStage, bad);
+      request(min(st + 2, s1 - 1));
+    }
+    if (t <= NG) s.odd[(st + 2) % 3][t] = 0;  // last read a barrier ago, written after the next
+    __syncthreads();
+  }
+  sum = xor32_add(sum);
+  if (col >= cols) return;
+  if (chunks == 1) {
+    const float inv = valid ? 1.0f / sum : nan;
+    float *out = a.out + ((size_t)(first + row) * a.num_heads + head) * HD + 4 * half;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float f = odd >> g & 1 ? nan : inv;
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *(float4 *)(out + 32 * g + 2 * i) = make_float4(o[g][i] * f, o[g][i + 1] * f, o[g][i + 2] * f, o[g][i + 3] * f);
+    }
+  } else {
+    float *rec = records + (size_t)record * (kTile * (HD + 2));
+    const int k = 32 * w + (l & 31);
+    if (half == 0) {
+      rec[2 * k] = ref;
+      rec[2 * k + 1] = sum;
+    }
+    float *out = rec + 2 * kTile + k * HD + 4 * half;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float f = odd >> g & 1 ? nan : 1.0f;
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *(float4 *)(out + 32 * g + 2 * i) = make_float4(o[g][i] * f, o[g][i + 1] * f, o[g][i + 2] * f, o[g][i + 3] * f);
+    }
+  }
+}
+
+// The chunks of cut tiles added up, weighted by 2^(reference - the largest):
+// HD / 4 threads a column, 32 columns a workgroup.
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_rows_merge_kernel(AttnArgs a, const int *header, const RowsTile *tiles,
+                                                             const float *records) {
+  constexpr int TPC = HD / 4;
+  const int G = a.num_heads / a.kv.heads;
+  if ((int)(blockIdx.x / 4) >= header[0]) return;
+  const RowsTile m = tiles[blockIdx.x / 4];
+  // the tile's run ends at its lane's rows
+  int lo = 0, hi = a.lanes - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.row_start[mid + 1] > m.row) hi = mid;
+    else lo = mid + 1;
+  }
+  const int first = a.row_start[lo], cols = (a.row_start[lo + 1] - first) * G;
+  for (int i = threadIdx.x; i < 32 * TPC; i += 256) {
+    const int k = 32 * (blockIdx.x & 3) + i / TPC, col = m.cols + k, d = i % TPC * 4;
+    if (col >= cols) break;
+    const float *rec = records + (size_t)m.record * (kTile * (HD + 2));
+    float top = kNoRef;
+    for (int c = 0; c < m.chunks; ++c) top = fmaxf(top, rec[(size_t)c * (kTile * (HD + 2)) + 2 * k]);
+    float sum = 0.0f;
+    float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < m.chunks; ++c) {
+      const float *p = rec + (size_t)c * (kTile * (HD + 2));
+      const float f = __builtin_amdgcn_exp2f(p[2 * k] - top);
+      const float4 x = *(const float4 *)(p + 2 * kTile + k * HD + d);
+      sum = fmaf(p[2 * k + 1], f, sum);
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      o.z = fmaf(x.z, f, o.z);
+      o.w = fmaf(x.w, f, o.w);
+    }
+    const int row = col / G, head = m.head * G + col - row * G;
+    *(float4 *)(a.out + ((size_t)(first + row) * a.num_heads + head) * HD + d) =
+        make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum);
+  }
+}
+
 }  // namespace
 }  // namespace gk
 
@@ -1114,7 +1547,7 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
   if (int rc = pool_view(pool, layer, &a.kv)) return rc;
   const uint64_t need = glacier_hip_kv4_attention_workspace_bytes(lanes, max_rows, num_heads,
                                                                   pool->num_kv_heads, pool->head_dim);
-  if (need == 0 || ws_bytes < need || max_ctx == 0 || max_ctx > (1u << 30) ||
+  if (need == 0 || ws_bytes < need || max_ctx == 0 || max_ctx > (1u << 26) ||
       max_ctx > (uint64_t)max_pages * gk::kPage ||
       (uint64_t)lanes * ((max_ctx + 15) / 16) * pool->num_kv_heads >= (1ull << 31))
     return GLACIER_HIP_SHAPE_MISMATCH;
@@ -1153,9 +1586,23 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
     GH_CHECK(ctx, hipGetLastError());
     return GLACIER_HIP_OK;
   }
-  const dim3 grid(max_rows, pool->num_kv_heads);
-  if (pool->head_dim == 128) gk::kv4_attn_kernel<128><<<grid, 256, 0, st>>>(a);
-  else gk::kv4_attn_kernel<64><<<grid, 256, 0, st>>>(a);
+  // workgroups a CU holds
+  const int slots = std::min(gk::kRowsSlots, ctx->props.multiProcessorCount * 2);
+  const int split = (max_ctx + gk::kStage - 1) / gk::kStage > (uint32_t)gk::kMinStages;
+  const uint64_t tiles = (uint64_t)max_rows * (num_heads / a.kv.heads) / gk::kTile + lanes;
+  // items at most: the tiles, and the chunks of those that are cut (a cut
+  // tile has more than three means of a slot in its longest, one and a half in all)
+  const uint32_t grid = (uint32_t)(tiles * a.kv.heads + (split ? gk::kRowsRecords : 0));
+  int *header = (int *)ws;
+  auto *cut = (gk::RowsTile *)((char *)ws + 256);
+  float *records = (float *)((char *)ws + gk::kRowsHeader);
+  if (pool->head_dim == 128) {
+    gk::kv4_rows_kernel<128><<<grid, 256, 0, st>>>(a, slots, split, header, cut, records);
+    if (split) gk::kv4_rows_merge_kernel<128><<<4 * gk::kRowsCut, 256, 0, st>>>(a, header, cut, records);
+  } else {
+    gk::kv4_rows_kernel<64><<<grid, 256, 0, st>>>(a, slots, split, header, cut, records);
+    if (split) gk::kv4_rows_merge_kernel<64><<<4 * gk::kRowsCut, 256, 0, st>>>(a, header, cut, records);
+  }
   GH_CHECK(ctx, hipGetLastError());
   return GLACIER_HIP_OK;
 }
@@ -1268,8 +1715,10 @@ uint64_t glacier_hip_kv4_attention_workspace_bytes(uint32_t lanes, uint32_t max_
       num_heads % num_kv_heads != 0 || num_heads / num_kv_heads == 0 ||
       num_heads / num_kv_heads > (uint32_t)gk::kMaxGroup)
     return 0;
-  return merge_bytes(lanes, num_kv_heads) +
-         (uint64_t)gk::kMaxRecords * gk::kMaxGroup * (head_dim + 2) * sizeof(float);
+  const uint64_t one = merge_bytes(lanes, num_kv_heads) +
+                       (uint64_t)gk::kMaxRecords * gk::kMaxGroup * (head_dim + 2) * sizeof(float);
+  const uint64_t runs = gk::kRowsHeader + (uint64_t)gk::kRowsRecords * gk::kTile * (head_dim + 2) * sizeof(float);
+  return std::max(one, runs);
 }
 
 int glacier_hip_paged_attention_kv4(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool,

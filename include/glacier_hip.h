@@ -483,7 +483,7 @@ int glacier_hip_kv4_read(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t 
  * ctx_lens_dev positions in f32 arithmetic on the stored values. A lane of
  * length 0 gets zeros; a length outside 0..max_ctx, or a page id of an
  * attended position outside the pool, makes the lane's output NaN.
- * num_heads / num_kv_heads <= 8; max_ctx <= 16 * max_pages_per_lane; q_dev,
+ * num_heads / num_kv_heads <= 8; max_ctx <= 16 * max_pages_per_lane and 2^26; q_dev,
  * out_dev (which must not overlap) and workspace_dev 16-byte aligned.
  * workspace_dev holds glacier_hip_kv4_attention_workspace_bytes(lanes, lanes,
  * num_heads, num_kv_heads, head_dim) bytes, zero before its first call; each
