@@ -1021,6 +1021,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kTile = 128;        // columns of a workgroup
 constexpr int kStage = 32;        // keys of a stage
 constexpr int kMinStages = 8;     // stages of a chunk at least
+constexpr int kRowsRing = 4;      // stages whose pages are in LDS or on their way
 constexpr int kRowsSlots = 512;   // workgroups that a batch is cut for, at most
 // A cut tile's longest is over Q = 3 means of a slot, and its lane's tiles
 // average half of it: fewer than slots / 1.5 are cut, into 4 / 3 slots chunks.
@@ -1030,10 +1031,12 @@ constexpr size_t kRowsHeader = 16384;  // workspace: the cut tiles' count and pl
 template <int HD>
 struct RowsLds {
   // [step][high, low][lane] operands of K, [32 dims][16 keys][high, low][lane] of V
-  uint8_t k[2][HD / 16][2][1024], v[2][HD / 32][2][2][1024];
+  uint8_t k[HD / 16][2][1024], v[HD / 32][2][2][1024];
+  Slot<HD> ring[kRowsRing];  // the pages of the stages ahead
+  int bad[kRowsRing];        // which of a slot's two pages lie outside the pool
   // keys whose V group is no number, by group, and whether there are any: of
-  // the stage in use, the next, and one to clear
-  uint32_t odd[3][HD / 32 + 1];
+  // this stage and the one before
+  uint32_t odd[2][HD / 32 + 1];
   int item[8];
 };
 
@@ -1130,32 +1133,43 @@ static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int
   return m;
 }
 
-// What a thread requests of a stage: waves 0 and 1 K codes of a (page,
-// position, chunk c of 8 dims a group), waves 2 and 3 V codes of a (page, four
-// positions c, column j).
+// What a thread turns into values of a stage: GPT = HD / 64 groups (those of
+// half t / 128) of a K chunk (page, position, 8 dims c of a group) or of a V
+// chunk (page, four positions c, column j).
 template <int HD>
-struct Raw {
-  uint32_t code[HD / 32];
-  uint32_t step[HD / 16], low[HD / 16];
+struct RawKeys {
+  uint32_t code[HD / 64], step[HD / 64], low[HD / 64];
+};
+template <int HD>
+struct RawValues {
+  uint32_t code[2], step[HD / 32], low[HD / 32];
 };
 
 template <int HD>
-static __device__ __forceinline__ void load_raw(Raw<HD> &r, const uint8_t *tile, int w, int l) {
-  constexpr int NG = HD / 32;
-  const int c = l >> 4, j = l & 15;
-  if (w < 2) {
-    load_words(r.code, tile + j * (HD / 2) + c * (4 * NG));
+static __device__ __forceinline__ RawKeys<HD> raw_keys(const Slot<HD> &s, int page, int part, int l) {
+  constexpr int NG = HD / 32, GPT = HD / 64;
+  const int c = l >> 4, j = l & 15, g0 = part * GPT;
+  RawKeys<HD> r;
+  load_words(r.code, s.kc[page] + (HD == 128 ? l * 16 : j * 32 + c * 8) + g0 * 4);
 #pragma unroll
-    for (int g = 0; g < NG; ++g)
-      r.step[g] = *(const uint16_t *)(tile + 8 * HD + 2 * ((j >> 2) * (4 * NG) + g * 4 + (j & 3)));
-    const uint8_t *p = tile + 9 * HD + j * (2 * NG);
-#pragma unroll
-    for (int g = 0; g < NG; g += 2) r.low[g / 2] = *(const uint32_t *)(p + 2 * g);
-  } else {
-    load_words(r.code, tile + (c * 16 + j) * (4 * NG));
-    load_words(r.step, tile + 8 * HD + c * (8 * NG));
-    load_words(r.low, tile + 9 * HD + c * (8 * NG));
+  for (int g = 0; g < GPT; ++g) {
+    r.step[g] = *(const uint16_t *)(s.meta[page] + 2 * ((j >> 2) * (4 * NG) + (g0 + g) * 4 + (j & 3)));
+    r.low[g] = *(const uint16_t *)(s.meta[page] + HD + 2 * (j * NG + g0 + g));
   }
+  return r;
+}
+template <int HD>
+static __device__ __forceinline__ RawValues<HD> raw_values(const Slot<HD> &s, int page, int part, int l) {
+  constexpr int NG = HD / 32, GPT = HD / 64;
+  const int c = l >> 4, g0 = part * GPT;
+  RawValues<HD> r;
+  // unit h = the half of a position pair's words
+#pragma unroll
+  for (int pr = 0; pr < 2; ++pr)
+    r.code[pr] = *(const uint32_t *)(s.vc[page] + l * (4 * NG) + (pr * (HD / 64) + (HD == 128 ? part : 0)) * 4);
+  load_words(r.step, s.meta[page] + 2 * HD + (c * NG + g0) * 8);
+  load_words(r.low, s.meta[page] + 3 * HD + (c * NG + g0) * 8);
+  return r;
 }
 
 // fp16 high and low parts of two values: the high one truncated, so that the
@@ -1167,73 +1181,98 @@ static __device__ __forceinline__ void two_parts(float x, float y, uint32_t &hig
   low = __builtin_bit_cast(uint32_t, v2h{(_Float16)rx, (_Float16)ry});
 }
 
-// Stage st from the raw codes; keys: the stage's keys inside the context.
+// The words become unknown to the compiler, which would move what both arms
+// of a branch compute from them ahead of it, out of the matrix products' shadow.
+template <int N>
+static __device__ __forceinline__ void keep_here(uint32_t (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(w[i]));
+}
+
+// V positions past the context (left of the thread's four are inside), of no
+// page or with no number become zeros; the last are noted for their groups,
+// so that they reach the rows that see them and no others.
 template <int HD>
-static __device__ __forceinline__ void write_stage(RowsLds<HD> &s, int st, const Raw<HD> &r, int w, int l,
-                                                   int keys, bool bad) {
-  constexpr int NG = HD / 32;
-  const int c = l >> 4, j = l & 15, page = w & 1, buf = st & 1;
-  if (w < 2) {
-    const int key = 16 * page + j;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const float step = bad ? __uint_as_float(0x7FC00000u) : half_of(r.step[g], 0);
-      const float low = half_of(r.low[g >> 1], g & 1);
-      const uint32_t even = r.code[g] & 0x0F0F0F0Fu, odd = r.code[g] >> 4 & 0x0F0F0F0Fu;
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        two_parts(fmaf((float)(even >> 8 * i & 0xFFu), step, low), fmaf((float)(odd >> 8 * i & 0xFFu), step, low),
-                  hi[i], lo[i]);
-      const int at = (32 * (c & 1) + key) * 16;
-      *(uint4 *)(s.k[buf][2 * g + (c >> 1)][0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *(uint4 *)(s.k[buf][2 * g + (c >> 1)][1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-    return;
-  }
-  const int left = keys - 16 * page - 4 * c;  // of the thread's four positions
+static __device__ __forceinline__ void clean_values(uint32_t *notes, RawValues<HD> &r, int page, int part, int l,
+                                                    int keys, bool bad) {
+  constexpr int NG = HD / 32, GPT = HD / 64;
+  const int c = l >> 4, left = keys - 16 * page - 4 * c;
   uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < 2 * NG; ++i) most = max2(most, max2(r.step[i] & 0x7FFF7FFFu, r.low[i] & 0x7FFF7FFFu));
-  const bool odd = bad || left < 4 || (most & 0xFFFFu) >= 0x7C00u || most >> 16 >= 0x7C00u;
+  for (int i = 0; i < 2 * GPT; ++i) most = max2(most, max2(r.step[i] & 0x7FFF7FFFu, r.low[i] & 0x7FFF7FFFu));
+  if (!__any(bad || left < 4 || max2(most, 0x7BFF7BFFu) != 0x7BFF7BFFu)) return;
 #pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    float step[4], low[4];
+  for (int g = 0; g < GPT; ++g)
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      step[p] = half_of(r.step[2 * g + (p >> 1)], p & 1);
-      low[p] = half_of(r.low[2 * g + (p >> 1)], p & 1);
-    }
-    if (__any(odd)) {
-      // positions past the context, of no page, or with no number: zeros, the last noted
-      asm volatile("");
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const bool none = bad || p >= left, nan = !(fabsf(step[p]) <= 65504.0f && fabsf(low[p]) <= 65504.0f);
-        if (none || nan) step[p] = low[p] = 0.0f;
-        if (nan && !none && j == 0) {
-          atomicOr(&s.odd[st % 3][g], 1u << (16 * page + 4 * c + p));
-          atomicOr(&s.odd[st % 3][NG], 1u);
-        }
+      const int i = 2 * g + (p >> 1), sh = 16 * (p & 1);
+      const bool none = bad || p >= left;
+      const bool nan = (r.step[i] >> sh & 0x7C00u) == 0x7C00u || (r.low[i] >> sh & 0x7C00u) == 0x7C00u;
+      if (none || nan) {
+        r.step[i] &= ~(0xFFFFu << sh);
+        r.low[i] &= ~(0xFFFFu << sh);
+      }
+      if (nan && !none && (l & 15) == 0) {
+        atomicOr(&notes[part * GPT + g], 1u << (16 * page + 4 * c + p));
+        atomicOr(&notes[NG], 1u);
       }
     }
-    // blocks 2 g, 2 g + 1: byte g % 2 of unit g / 2 of each position
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      float x[4];
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const uint32_t word = r.code[(p >> 1) * (HD / 64) + (g >> 1)];
-        x[p] = fmaf((float)(word >> (16 * (p & 1) + 8 * (g & 1) + 4 * b) & 15u), step[p], low[p]);
-      }
-      uint32_t hi[2], lo[2];
-      two_parts(x[0], x[1], hi[0], lo[0]);
-      two_parts(x[2], x[3], hi[1], lo[1]);
-      const int at = (32 * (c & 1) + 16 * b + j) * 16 + (c >> 1) * 8;
-      *(uint2 *)(s.v[buf][g][page][0] + at) = make_uint2(hi[0], hi[1]);
-      *(uint2 *)(s.v[buf][g][page][1] + at) = make_uint2(lo[0], lo[1]);
-    }
+}
+
+// The thread's K or V values as operands, a part at a time so that a few
+// vector instructions can go between matrix products. K: two values of a
+// group (part n of 4 GPT), the fourth two write the chunk.
+template <int HD>
+struct KeyChunk {
+  uint32_t even, odd, hi[4], lo[4];
+};
+template <int HD>
+static __device__ __forceinline__ void key_part(RowsLds<HD> &s, const RawKeys<HD> &r, KeyChunk<HD> &o, int n, int page,
+                                                int part, int l, bool bad) {
+  const int i = n >> 2, k = n & 3;
+  if (k == 0) {
+    o.even = r.code[i] & 0x0F0F0F0Fu;
+    o.odd = r.code[i] >> 4 & 0x0F0F0F0Fu;
   }
+  const float step = bad ? __uint_as_float(0x7FC00000u) : half_of(r.step[i], 0), low = half_of(r.low[i], 0);
+  two_parts(fmaf((float)(o.even >> 8 * k & 0xFFu), step, low), fmaf((float)(o.odd >> 8 * k & 0xFFu), step, low),
+            o.hi[k], o.lo[k]);
+  if (k < 3) return;
+  const int c = l >> 4, j = l & 15, at = (32 * (c & 1) + 16 * page + j) * 16, g = part * (HD / 64) + i;
+  *(uint4 *)(s.k[2 * g + (c >> 1)][0] + at) = make_uint4(o.hi[0], o.hi[1], o.hi[2], o.hi[3]);
+  *(uint4 *)(s.k[2 * g + (c >> 1)][1] + at) = make_uint4(o.lo[0], o.lo[1], o.lo[2], o.lo[3]);
+}
+// V: block b of 16 dims of a group, part n of 2 GPT.
+template <int HD>
+static __device__ __forceinline__ void value_part(RowsLds<HD> &s, const RawValues<HD> &r, int n, int page, int part,
+                                                  int l) {
+  const int i = n >> 1, b = n & 1, c = l >> 4, j = l & 15, g = part * (HD / 64) + i;
+  // blocks 2 g, 2 g + 1: byte g % 2 of each position's half word
+  float x[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const uint32_t w = r.code[p >> 1] >> (HD == 128 ? 8 * i : 8 * part);
+    x[p] = fmaf((float)(w >> (16 * (p & 1) + 4 * b) & 15u), half_of(r.step[2 * i + (p >> 1)], p & 1),
+                half_of(r.low[2 * i + (p >> 1)], p & 1));
+  }
+  uint32_t hi[2], lo[2];
+  two_parts(x[0], x[1], hi[0], lo[0]);
+  two_parts(x[2], x[3], hi[1], lo[1]);
+  const int at = (32 * (c & 1) + 16 * b + j) * 16 + (c >> 1) * 8;
+  *(uint2 *)(s.v[g][page][0] + at) = make_uint2(hi[0], hi[1]);
+  *(uint2 *)(s.v[g][page][1] + at) = make_uint2(lo[0], lo[1]);
+}
+template <int HD>
+static __device__ __forceinline__ void write_keys(RowsLds<HD> &s, const RawKeys<HD> &r, int page, int part, int l,
+                                                  bool bad) {
+  KeyChunk<HD> o;
+#pragma unroll
+  for (int n = 0; n < HD / 16; ++n) key_part(s, r, o, n, page, part, l, bad);
+}
+template <int HD>
+static __device__ __forceinline__ void write_values(RowsLds<HD> &s, const RawValues<HD> &r, int page, int part, int l) {
+#pragma unroll
+  for (int n = 0; n < HD / 32; ++n) value_part(s, r, n, page, part, l);
 }
 
 template <int HD>
@@ -1258,7 +1297,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
       if (blockIdx.x == 0 && split) header[0] = cut;
     }
   }
-  if (t < 3 * (NG + 1)) s.odd[t / (NG + 1)][t % (NG + 1)] = 0;
+  if (t < 2 * (NG + 1)) s.odd[t / (NG + 1)][t % (NG + 1)] = 0;
   __syncthreads();
   const int lane = __builtin_amdgcn_readfirstlane(s.item[0]);
   if (lane < 0) return;
@@ -1324,45 +1363,81 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
   float ref = kNoRef, sum = 0.0f;
   int odd = 0;  // groups of this column with no number
   const bool wave_in = kTile * tile + 32 * w < cols;
-  const int wave_first = __builtin_amdgcn_readfirstlane(seen);  // the fewest and most keys of the wave's columns
-  const int wave_last = __builtin_amdgcn_readlane(seen, 31);
+  const int wave_first = __builtin_amdgcn_readfirstlane(seen);  // the fewest keys of the wave's columns
 
   const int32_t *table = a.table + (size_t)lane * a.max_pages;
   const int pages = (ctx + kPage - 1) / kPage;
-  const size_t mine = (size_t)(2 * h + (w >> 1)) * (10 * HD);
+  const uint8_t *head_base = a.kv.base + (size_t)(2 * h) * (10 * HD);
+  const int page = w & 1, part = w >> 1;
   int id_base = -64;
   uint32_t ids = 0;
-  bool bad = false;
-  Raw<HD> raw;
-  auto request = [&](int st) {  // this wave's page of a stage
-    const int p = 2 * st + (w & 1);
-    if (2 * st >= id_base + 64) {
-      id_base = 2 * st;
-      ids = (uint32_t)table[min(id_base + l, pages - 1)];
+  // stage s0 + i into its slot, by wave i % kRowsRing
+  auto request = [&](int i) {
+    const int p = 2 * (s0 + i);
+    if (p >= id_base + 64) {
+      id_base = p;
+      ids = (uint32_t)table[min(p + l, pages - 1)];
     }
-    const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)ids, min(p, pages - 1) - id_base);
-    bad = id >= a.kv.page_count;
-    load_raw(raw, a.kv.base + (size_t)(bad ? 0 : id) * a.kv.page_bytes + mine, w, l);
+    uint32_t id[2];
+    int bad = 0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      id[x] = (uint32_t)__builtin_amdgcn_readlane((int)ids, min(p + x, pages - 1) - id_base);
+      if (id[x] >= a.kv.page_count) {
+        bad |= 1 << x;
+        id[x] = 0;
+      }
+    }
+    if (l == 0) s.bad[i % kRowsRing] = bad;
+    copy_pair(&s.ring[i % kRowsRing], head_base + id[0] * a.kv.page_bytes, head_base + id[1] * a.kv.page_bytes, l);
   };
-  if (s0 < s1) {
-    request(s0);
-    write_stage(s, s0, raw, w, l, ctx - s0 * kStage, bad);
-    request(min(s0 + 1, s1 - 1));
-  }
+  const int stages = s1 - s0;
+  if (w < kRowsRing - 1 && w < stages) request(w);
+  arrive<0>();
   __syncthreads();
-  for (int st = s0; st < s1; ++st) {
-    const int buf = st & 1, key0 = st * kStage;
-    if (wave_in && key0 < wave_last) {
+  if (stages > 0) write_keys(s, raw_keys(s.ring[0], page, part, l), page, part, l, s.bad[0] >> page & 1);
+  __syncthreads();
+  for (int st = 0; st < stages; ++st) {
+    const int key0 = (s0 + st) * kStage;
+    if (w == (st + 3) % kRowsRing && st + 3 < stages) request(st + 3);
+    // scores, and between the matrix products this stage's values
+    RawValues<HD> rv = raw_values(s.ring[st % kRowsRing], page, part, l);
+    if (t <= NG) s.odd[(st + 1) & 1][t] = 0;  // read before the last barrier, written after the next
+    clean_values(s.odd[st & 1], rv, page, part, l, ctx - key0, s.bad[st % kRowsRing] >> page & 1);
+    uint32_t ph[8], pl[8];
+    if (wave_in) {
+      keep_here(rv.code);
       f16v sc;
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+      // (two sums in turn: a product that adds to the one before it waits for it)
+      f16v sd;
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const v8h kh = *(const v8h *)(s.k[buf][i][0] + l * 16), kl = *(const v8h *)(s.k[buf][i][1] + l * 16);
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[i], sc, 0, 0, 0);
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[i], sc, 0, 0, 0);
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[i], sc, 0, 0, 0);
+      for (int i = 0; i < 16; ++i) sd[i] = 0.0f;
+      v8h kh[4], kl[4];
+      auto read_k = [&](int i) {
+        kh[i & 3] = *(const v8h *)(s.k[i][0] + l * 16);
+        kl[i & 3] = *(const v8h *)(s.k[i][1] + l * 16);
+      };
+      read_k(0);
+      read_k(1);
+#pragma unroll
+      for (int i = 0; i < S; i += 2) {
+        if (i + 2 < S) {
+          read_k(i + 2);
+          read_k(i + 3);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (the next operands before this step's products)
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[i & 3], ql[i], sc, 0, 0, 0);
+        sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[i + 1 & 3], ql[i + 1], sd, 0, 0, 0);
+        value_part(s, rv, i / 2, page, part, l);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[i & 3], qh[i], sc, 0, 0, 0);
+        sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[i + 1 & 3], qh[i + 1], sd, 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[i & 3], qh[i], sc, 0, 0, 0);
+        sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[i + 1 & 3], qh[i + 1], sd, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      sc += sd;
       if (key0 + kStage > wave_first) {
         asm volatile("");
 #pragma unroll
@@ -1376,8 +1451,8 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
       if (__any(fmaf(top, mult, -ref) > kSlack)) {
         asm volatile("");
         const float high = xor32_max(top) * mult;
-        const float next = high - ref > kSlack ? high : ref, f = exp2f(ref - next);
-        ref = next;
+        const float above = high - ref > kSlack ? high : ref, f = exp2f(ref - above);
+        ref = above;
         sum *= f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) o[g] *= f;
@@ -1388,33 +1463,56 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
         sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], mult, shift));
         sum += sc[i];
       }
-      uint32_t ph[8], pl[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) two_parts(sc[2 * i], sc[2 * i + 1], ph[i], pl[i]);
+    } else {
+      write_values(s, rv, page, part, l);
+    }
+    if (w == (st + 1) % kRowsRing) arrive<0>();  // the next stage, asked for two and a half ago
+    __syncthreads();
+    // output, and between the matrix products the next stage's keys (past the
+    // last one what the slot holds, which nothing reads)
+    RawKeys<HD> rk = raw_keys(s.ring[(st + 1) % kRowsRing], page, part, l);
+    const bool bad = s.bad[(st + 1) % kRowsRing] >> page & 1;
+    if (wave_in) {
+      keep_here(rk.code);
+      KeyChunk<HD> kc;
+      v8h vh[4], vl[4];
+      auto read_v = [&](int i) {
+        vh[i & 3] = *(const v8h *)(s.v[i % NG][i / NG][0] + l * 16);
+        vl[i & 3] = *(const v8h *)(s.v[i % NG][i / NG][1] + l * 16);
+      };
+      read_v(0);
+      read_v(1);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int i = 0; i < 2 * NG; i += 2) {
+        const int x = i / NG, g = i % NG;
+        if (i + 2 < 2 * NG) {
+          read_v(i + 2);
+          read_v(i + 3);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         const v8h bh = as_v8h(ph[4 * x], ph[4 * x + 1], ph[4 * x + 2], ph[4 * x + 3]);
         const v8h bl = as_v8h(pl[4 * x], pl[4 * x + 1], pl[4 * x + 2], pl[4 * x + 3]);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const v8h vh = *(const v8h *)(s.v[buf][g][x][0] + l * 16), vl = *(const v8h *)(s.v[buf][g][x][1] + l * 16);
-          o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, bl, o[g], 0, 0, 0);
-          o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, bh, o[g], 0, 0, 0);
-          o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, bh, o[g], 0, 0, 0);
-        }
+        o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[i & 3], bl, o[g], 0, 0, 0);
+        o[g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[i + 1 & 3], bl, o[g + 1], 0, 0, 0);
+        key_part(s, rk, kc, i, page, part, l, bad);
+        o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl[i & 3], bh, o[g], 0, 0, 0);
+        o[g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl[i + 1 & 3], bh, o[g + 1], 0, 0, 0);
+        key_part(s, rk, kc, i + 1, page, part, l, bad);
+        o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[i & 3], bh, o[g], 0, 0, 0);
+        o[g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[i + 1 & 3], bh, o[g + 1], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (__builtin_amdgcn_readfirstlane(s.odd[st % 3][NG])) {
+      if (__builtin_amdgcn_readfirstlane(s.odd[st & 1][NG])) {
         const int k = min(kStage, seen - key0);
         const uint32_t shown = k <= 0 ? 0u : k >= 32 ? 0xFFFFFFFFu : (1u << k) - 1;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) odd |= (s.odd[st % 3][g] & shown) != 0 ? 1 << g : 0;
+        for (int g = 0; g < NG; ++g) odd |= (s.odd[st & 1][g] & shown) != 0 ? 1 << g : 0;
       }
+    } else {
+      write_keys(s, rk, page, part, l, bad);
     }
-    if (st + 1 < s1) {
-      write_stage(s, st + 1, raw, w, l, ctx - (st + 1) * kStage, bad);
-      request(min(st + 2, s1 - 1));
-    }
-    if (t <= NG) s.odd[(st + 2) % 3][t] = 0;  // last read a barrier ago, written after the next
     __syncthreads();
   }
   sum = xor32_add(sum);
