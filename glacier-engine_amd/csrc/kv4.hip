@@ -1023,9 +1023,7 @@ constexpr int kStage = 32;        // keys of a stage
 constexpr int kMinStages = 8;     // stages of a chunk at least
 constexpr int kRowsRing = 4;      // stages whose pages are in LDS or on their way
 constexpr int kRowsSlots = 512;   // workgroups that a batch is cut for, at most
-// A cut tile's longest is over Q = 3 means of a slot, and its lane's tiles
-// average half of it: fewer than slots / 1.5 are cut, into 4 / 3 slots chunks.
-constexpr int kRowsCut = kRowsSlots * 2 / 3 + 8, kRowsRecords = kRowsSlots * 4 / 3 + 16;
+constexpr int kRowsRecords = kRowsSlots;  // chunks of cut tiles at most
 constexpr size_t kRowsHeader = 16384;  // workspace: the cut tiles' count and places, then records
 
 template <int HD>
@@ -1044,7 +1042,7 @@ struct RowsItem {
   int lane, head, tile, chunk, chunks, record, split;  // lane < 0: none
 };
 struct RowsTile {  // a cut tile, for the merge
-  int row, head, cols, chunks, record;
+  int first, head, col, cols, chunks, record;  // its run's first row, its first column of the run's
 };
 
 static __device__ __forceinline__ float wave_scan_f(float v) {
@@ -1061,39 +1059,62 @@ static __device__ __forceinline__ float wave_scan_f(float v) {
 static __device__ __forceinline__ void run_of(const AttnArgs &a, int lane, int &first, int &n) {
   first = lane < a.lanes ? a.row_start[lane] : 0;
   const int end = lane < a.lanes ? a.row_start[lane + 1] : 0;
-  n = first >= 0 && end <= a.max_rows ? max(0, end - first) : 0;
+  n = first >= 0 && first < end && end <= a.max_rows ? end - first : 0;  // (no difference that wraps)
 }
 
 // Work items: (lane, tile, KV head, chunk), the tiles of a lane from its last
 // on (the longest), by one wave; a thread holds lanes / 64 lanes. A lane's
-// tiles are cut into as many chunks as its longest has shares Q of the
-// batch's stages, a share three times the mean of a slot (tiles of a prompt
-// average half their longest: a prompt that fills the device stays whole).
+// tiles are cut into as many chunks as its longest has shares Q of stages: the
+// smallest Q of a few multiples of a slot's mean that leaves no more items
+// than slots, or than the tiles and half the slots more. (A prompt that fills
+// the device with whole tiles so stays whole: 2048 rows cut in two took 151 us
+// instead of 133, 512 rows at the end of 4096 117 instead of 138.)
 // The list is dealt in runs of 256 (a CU each), every other one backwards, so
 // that CUs pair long items with short ones.
 static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int slots, bool split, int l,
                                                           int *cut_tiles) {
   const int per = (a.lanes + 63) / 64, Hkv = a.kv.heads, G = a.num_heads / Hkv;
-  auto tiles_of = [&](int i, int &stages) {
-    int first, n;
+  auto tiles_of = [&](int i, int &stages, int &n) {
+    int first;
     run_of(a, l * per + i, first, n);
     const int ctx = n > 0 ? a.ctx[l * per + i] : 0;
     stages = ctx >= n && ctx <= a.max_ctx ? (ctx + kStage - 1) / kStage : 0;
     return (n * G + kTile - 1) / kTile;
   };
-  float work = 0.0f;
-  for (int i = 0; i < per; ++i) {
-    int st, first, n;
-    const int tiles = tiles_of(i, st);
-    run_of(a, l * per + i, first, n);
-    work += (float)tiles * ((float)st - 0.5f * (float)n / kStage);
+  int n0, st0;
+  const int tiles0 = tiles_of(0, st0, n0);
+  int Q = 1 << 30;
+  if (split) {
+    float work = (float)tiles0 * ((float)st0 - 0.5f * (float)n0 / kStage);
+    for (int i = 1; i < per; ++i) {
+      int st, n;
+      const int tiles = tiles_of(i, st, n);
+      work += (float)tiles * ((float)st - 0.5f * (float)n / kStage);
+    }
+    work = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_scan_f(work)), 63)) * (float)Hkv;
+    auto items_of = [&](int q) {
+      int items = tiles0 * max(1, (st0 + q - 1) / q);
+      for (int i = 1; i < per; ++i) {
+        int st, n;
+        const int tiles = tiles_of(i, st, n);
+        items += tiles * max(1, (st + q - 1) / q);
+      }
+      return __builtin_amdgcn_readlane(wave_scan_dpp(items), 63) * Hkv;
+    };
+    const int room = max(slots, items_of(Q) + slots / 2);
+    for (int k = 4; k <= 16; k += 2) {  // quarters of the mean
+      const int q = max(kMinStages, (int)(work * (float)k / (4.0f * (float)slots)) + 1);
+      if (items_of(q) <= room) {
+        Q = q;
+        break;
+      }
+    }
   }
-  const float total = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_scan_f(work)), 63)) * (float)Hkv;
-  const int Q = split ? max(kMinStages, (int)(3.0f * total / (float)slots) + 1) : 1 << 30;
-  int count = 0, cut = 0, cut_items = 0;
+  int count = 0, cut = 0, cut_items = 0, rows = 0;
   for (int i = 0; i < per; ++i) {
-    int st;
-    const int tiles = tiles_of(i, st), chunks = max(1, (st + Q - 1) / Q);
+    int st = st0, n = n0;
+    const int tiles = i == 0 ? tiles0 : tiles_of(i, st, n), chunks = max(1, (st + Q - 1) / Q);
+    rows += n;
     count += tiles * Hkv * chunks;
     if (chunks > 1) {
       cut += tiles * Hkv;
@@ -1101,8 +1122,11 @@ static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int
     }
   }
   const int last = wave_scan_dpp(count), cut_last = wave_scan_dpp(cut), rec_last = wave_scan_dpp(cut_items);
-  const int all = __builtin_amdgcn_readlane(last, 63);
-  *cut_tiles = __builtin_amdgcn_readlane(cut_last, 63);
+  // runs of more rows than there are (they overlap) have no items: the grid
+  // holds those of max_rows rows
+  const bool fits = __builtin_amdgcn_readlane(wave_scan_dpp(rows), 63) <= a.max_rows;
+  const int all = fits ? __builtin_amdgcn_readlane(last, 63) : 0;
+  *cut_tiles = fits ? __builtin_amdgcn_readlane(cut_last, 63) : 0;
   RowsItem m{-1, 0, 0, 0, 0, 0, 0};
   int item = blockIdx.x;
   if (item >= all) return m;
@@ -1320,7 +1344,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
   const int all = valid ? (ctx - n + tile_row + 1 + kStage - 1) / kStage : 0;
   const int s0 = chunk_first(chunk, all, chunks), s1 = chunk_first(chunk + 1, all, chunks);
   if (split && chunks > 1 && chunk == 0 && t == 0)
-    tiles[s.item[6]] = {first + kTile * tile / G, h, kTile * tile, chunks, record};
+    tiles[s.item[6]] = {first, h, kTile * tile, cols, chunks, record};
 
   // queries: q log2(e) / sqrt(HD) = 2^e q', the largest |q'| of a column in
   // [2^13, 2^14), as the B operand in two fp16 parts
@@ -1546,43 +1570,78 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
 }
 
 // The chunks of cut tiles added up, weighted by 2^(reference - the largest):
-// HD / 4 threads a column, 32 columns a workgroup.
+// HD / 4 threads for a column (of many chunks: for one of kParts shares of
+// them, which meet in LDS), four chunks' loads on their way at a time. The
+// time is a chain of dependent loads: one thread for all chunks of a column,
+// in two passes, took 17.5 us at 42 chunks where this takes MERGE_US.
+constexpr int kParts = 4, kMergeGrid = 2048;
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_rows_merge_kernel(AttnArgs a, const int *header, const RowsTile *tiles,
                                                              const float *records) {
-  constexpr int TPC = HD / 4;
-  const int G = a.num_heads / a.kv.heads;
-  if ((int)(blockIdx.x / 4) >= header[0]) return;
-  const RowsTile m = tiles[blockIdx.x / 4];
-  // the tile's run ends at its lane's rows
-  int lo = 0, hi = a.lanes - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a.row_start[mid + 1] > m.row) hi = mid;
-    else lo = mid + 1;
-  }
-  const int first = a.row_start[lo], cols = (a.row_start[lo + 1] - first) * G;
-  for (int i = threadIdx.x; i < 32 * TPC; i += 256) {
-    const int k = 32 * (blockIdx.x & 3) + i / TPC, col = m.cols + k, d = i % TPC * 4;
-    if (col >= cols) break;
-    const float *rec = records + (size_t)m.record * (kTile * (HD + 2));
-    float top = kNoRef;
-    for (int c = 0; c < m.chunks; ++c) top = fmaxf(top, rec[(size_t)c * (kTile * (HD + 2)) + 2 * k]);
-    float sum = 0.0f;
+  constexpr int TPC = HD / 4, SUBS = 256 / TPC;
+  constexpr size_t REC = kTile * (HD + 2);
+  __shared__ float4 acc[256];
+  __shared__ float2 stat[256 / TPC];
+  const int G = a.num_heads / a.kv.heads, cut = header[0], d = threadIdx.x % TPC * 4;
+  for (int u = blockIdx.x; u < cut * (kTile / SUBS * kParts); u += gridDim.x) {
+    const int unit = u / cut;
+    const RowsTile m = tiles[u - unit * cut];
+    // shares of a column's chunks, and this thread's column and share
+    const int parts = m.chunks > 4 ? kParts : 1, part = threadIdx.x / TPC % parts;
+    const int k0 = unit * (SUBS / parts), k = k0 + threadIdx.x / TPC / parts, col = m.col + k;
+    if (k0 >= kTile || m.col + k0 >= m.cols) continue;  // (the whole workgroup)
+    // past the run a record holds nothing: the last column again, not written
+    const int kc = min(k, m.cols - 1 - m.col);
+    const float *rec = records + m.record * REC;
+    float top = kNoRef, sum = 0.0f;
     float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c = 0; c < m.chunks; ++c) {
-      const float *p = rec + (size_t)c * (kTile * (HD + 2));
-      const float f = __builtin_amdgcn_exp2f(p[2 * k] - top);
-      const float4 x = *(const float4 *)(p + 2 * kTile + k * HD + d);
-      sum = fmaf(p[2 * k + 1], f, sum);
-      o.x = fmaf(x.x, f, o.x);
-      o.y = fmaf(x.y, f, o.y);
-      o.z = fmaf(x.z, f, o.z);
-      o.w = fmaf(x.w, f, o.w);
+    for (int i = part; i < m.chunks; i += 4 * parts) {
+      float2 rs[4];
+      float4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float *p = rec + (size_t)min(i + j * parts, m.chunks - 1) * REC;
+        rs[j] = *(const float2 *)(p + 2 * kc);
+        x[j] = *(const float4 *)(p + 2 * kTile + kc * HD + d);
+      }
+      float high = top;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j * parts < m.chunks) high = fmaxf(high, rs[j].x);
+      const float f = __builtin_amdgcn_exp2f(top - high);
+      top = high;
+      sum *= f;
+      o = {o.x * f, o.y * f, o.z * f, o.w * f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j * parts < m.chunks) {
+          const float g = __builtin_amdgcn_exp2f(rs[j].x - top);
+          sum = fmaf(rs[j].y, g, sum);
+          o = {fmaf(x[j].x, g, o.x), fmaf(x[j].y, g, o.y), fmaf(x[j].z, g, o.z), fmaf(x[j].w, g, o.w)};
+        }
     }
-    const int row = col / G, head = m.head * G + col - row * G;
-    *(float4 *)(a.out + ((size_t)(first + row) * a.num_heads + head) * HD + d) =
-        make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum);
+    if (parts > 1) {
+      acc[threadIdx.x] = o;
+      if (d == 0) stat[threadIdx.x / TPC] = {top, sum};
+      __syncthreads();
+      if (part == 0)
+#pragma unroll
+        for (int j = 1; j < kParts; ++j) {
+          const float2 rs = stat[threadIdx.x / TPC + j];
+          const float4 x = acc[threadIdx.x + j * TPC];
+          const float high = fmaxf(top, rs.x), f = __builtin_amdgcn_exp2f(top - high);
+          const float g = __builtin_amdgcn_exp2f(rs.x - high);
+          top = high;
+          sum = fmaf(rs.y, g, sum * f);
+          o = {fmaf(x.x, g, o.x * f), fmaf(x.y, g, o.y * f), fmaf(x.z, g, o.z * f), fmaf(x.w, g, o.w * f)};
+        }
+      __syncthreads();
+    }
+    if (part == 0 && k < kTile && col < m.cols) {
+      const int row = col / G, head = m.head * G + col - row * G;
+      *(float4 *)(a.out + ((size_t)(m.first + row) * a.num_heads + head) * HD + d) =
+          make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum);
+    }
   }
 }
 
@@ -1688,18 +1747,20 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
   const int slots = std::min(gk::kRowsSlots, ctx->props.multiProcessorCount * 2);
   const int split = (max_ctx + gk::kStage - 1) / gk::kStage > (uint32_t)gk::kMinStages;
   const uint64_t tiles = (uint64_t)max_rows * (num_heads / a.kv.heads) / gk::kTile + lanes;
-  // items at most: the tiles, and the chunks of those that are cut (a cut
-  // tile has more than three means of a slot in its longest, one and a half in all)
-  const uint32_t grid = (uint32_t)(tiles * a.kv.heads + (split ? gk::kRowsRecords : 0));
+  if (tiles * a.kv.heads >= (1u << 30)) return GLACIER_HIP_SHAPE_MISMATCH;
+  // items at most. Chunks past the tiles' number are no more than slots less
+  // the tiles or half the slots: those of cut tiles are slots at most.
+  const uint32_t whole = (uint32_t)(tiles * a.kv.heads);
+  const uint32_t grid = split ? std::max<uint32_t>(slots, whole + slots / 2) : whole;
   int *header = (int *)ws;
   auto *cut = (gk::RowsTile *)((char *)ws + 256);
   float *records = (float *)((char *)ws + gk::kRowsHeader);
   if (pool->head_dim == 128) {
     gk::kv4_rows_kernel<128><<<grid, 256, 0, st>>>(a, slots, split, header, cut, records);
-    if (split) gk::kv4_rows_merge_kernel<128><<<4 * gk::kRowsCut, 256, 0, st>>>(a, header, cut, records);
+    if (split) gk::kv4_rows_merge_kernel<128><<<gk::kMergeGrid, 256, 0, st>>>(a, header, cut, records);
   } else {
     gk::kv4_rows_kernel<64><<<grid, 256, 0, st>>>(a, slots, split, header, cut, records);
-    if (split) gk::kv4_rows_merge_kernel<64><<<4 * gk::kRowsCut, 256, 0, st>>>(a, header, cut, records);
+    if (split) gk::kv4_rows_merge_kernel<64><<<gk::kMergeGrid, 256, 0, st>>>(a, header, cut, records);
   }
   GH_CHECK(ctx, hipGetLastError());
   return GLACIER_HIP_OK;

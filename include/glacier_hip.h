@@ -486,9 +486,9 @@ int glacier_hip_kv4_read(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t 
  * num_heads / num_kv_heads <= 8; max_ctx <= 16 * max_pages_per_lane and 2^26; q_dev,
  * out_dev (which must not overlap) and workspace_dev 16-byte aligned.
  * workspace_dev holds glacier_hip_kv4_attention_workspace_bytes(lanes, lanes,
- * num_heads, num_kv_heads, head_dim) bytes, zero before its first call; each
- * call leaves it ready for the next. Calls that may overlap (streams, replays
- * of two graphs) need a workspace each; a larger one serves smaller calls.
+ * num_heads, num_kv_heads, head_dim) bytes of any contents. Calls that may
+ * overlap (streams, replays of two graphs) need a workspace each; a larger one
+ * serves smaller calls.
  * Asynchronous on `stream`; launches only. */
 uint64_t glacier_hip_kv4_attention_workspace_bytes(uint32_t lanes, uint32_t max_rows,
                                                    uint32_t num_heads, uint32_t num_kv_heads,
@@ -507,7 +507,9 @@ int glacier_hip_paged_attention_kv4(glacier_hip_context *ctx, const glacier_hip_
  * row_start_dev[i + 1] + r, its own included; ctx_lens_dev counts the step's
  * rows, whose K/V are already stored. Rows past the last lane's are left as
  * they were; max_rows is the capacity of q_dev / out_dev. A lane with more
- * rows than positions gets NaN, as the invalid lengths and pages above.
+ * rows than positions gets NaN, as the invalid lengths and pages above. A run
+ * that leaves the max_rows rows has none; runs that overlap, with more rows
+ * than max_rows together, leave every row as it was.
  * Workspace for (lanes, max_rows). Asynchronous on `stream`; launches only. */
 int glacier_hip_paged_attention_kv4_rows(glacier_hip_context *ctx,
                                          const glacier_hip_kv4_pool_t *pool, uint32_t layer,

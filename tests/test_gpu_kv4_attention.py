@@ -385,6 +385,34 @@ def test_a_nan_value_stays_out_of_earlier_rows(gh, gctx, hd):
         assert np.array_equal(got[:, 7:], want[:, 7:]) and np.isfinite(got[:, :7, 32:]).all()
 
 
+def test_runs_that_do_not_lie_in_the_rows_leave_them(gh, gctx):
+    """Overlapping runs (together more rows than there are) write nothing, a run
+    outside the rows has none; the workspace needs no first value."""
+    import torch
+
+    rng = np.random.default_rng(16)
+    cache = Cache(rng, [3000, 2900, 40], 2, 64)
+    q = rng.standard_normal((50, 14, 64))
+    ws = workspace(gh, 3, 50, 14, 2, 64)
+    ws.fill_(255)
+    want = run_rows(gh, gctx, cache, q, [20, 29, 1], ws=ws)
+    for start, untouched in (([0, 40, 10, 50], slice(0, 50)), ([0, 50, 0, 50], slice(0, 50)),
+                             ([-9, 20, 49, 50], slice(0, 20)), ([0, 20, 49, 51], slice(49, 50)),
+                             ([0, 2 ** 31 - 1, -2 ** 31, 50], slice(0, 50)), ([-2 ** 31, 2 ** 31 - 1, 0, 0], slice(0, 50))):
+        sd = _dev(np.array(start, np.int32))
+        lens = _dev(np.array(cache.ctx, np.int32))
+        qd, out = _dev(q.astype(np.float32)), torch.full((50, 14 * 64), 5.0, device="cuda")
+        torch.cuda.synchronize()
+        gh.check(gh.lib().glacier_hip_paged_attention_kv4_rows(
+            gctx.h, cache.pool_t, LAYER, qd.data_ptr(), cache.td.data_ptr(), cache.table.shape[1], sd.data_ptr(),
+            lens.data_ptr(), 3, 50, 14, cache.table.shape[1] * 16, out.data_ptr(), ws.data_ptr(), ws.numel(), None),
+            "rows", gctx.h)
+        torch.cuda.synchronize()
+        got = out.cpu().numpy().reshape(50, 14, 64)
+        assert (got[untouched] == 5.0).all()
+    assert np.array_equal(run_rows(gh, gctx, cache, q, [20, 29, 1], ws=ws), want)
+
+
 # ---- together --------------------------------------------------------------------------
 def _serve(gh, gctx, seed, stream=None):
     """Three lanes through a prompt step and decode steps: plan, append, attend,
