@@ -153,18 +153,6 @@ struct Bf16 {
 template <>
 __device__ __forceinline__ float widen(Bf16 v) { return __uint_as_float((uint32_t)v.bits << 16); }
 
-// Byte of dim d of position P in a tile's codes, and whether it is the high nibble.
-template <int HD>
-static __device__ __forceinline__ int code_byte(int which, int P, int d, int &high) {
-  constexpr int NG = HD / 32, NH = HD / 64;
-  if (which == 0) {
-    high = d & 1;
-    return P * (HD / 2) + ((d % 32) / 8 * NG + d / 32) * 4 + d % 8 / 2;
-  }
-  const int e = d / 16;  // the value's block of 16 dims
-  high = e & 1;
-  return ((((P / 4) * 16 + d % 16) * 2 + P / 2 % 2) * NH + e / 4) * 4 + P % 2 * 2 + e % 4 / 2;
-}
 template <int HD>
 static __device__ __forceinline__ int step_byte(int P, int g) {
   return 8 * HD + 2 * ((P / 4) * (HD / 8) + g * 4 + P % 4);
@@ -174,67 +162,202 @@ static __device__ __forceinline__ int low_byte(int which, int P, int g) {
   return which ? step_byte<HD>(P, g) + HD : 9 * HD + 2 * (P * (HD / 32) + g);
 }
 
-// One thread a group of 32 dims of a row's K or V.
-template <int HD, class T>
+// Both kernels: a wave takes kRun rows of one KV head's K or V; neighbouring
+// waves take the heads of the same rows.
+template <int HD>
+constexpr int kRun = 512 / HD;
+struct StoreWave {
+  int row, head, which;  // the first row
+};
+template <int HD>
+static __device__ __forceinline__ StoreWave store_wave(int heads) {
+  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), unit = wave / heads;
+  return {unit / 2 * kRun<HD>, wave - unit * heads, unit & 1};
+}
+// A slot's page and position; position < 0: none.
+static __device__ __forceinline__ int place_of(const Kv4 &kv, const int64_t *slots, int r, int rows, uint32_t &page) {
+  const uint64_t slot = r < rows ? (uint64_t)slots[r] : ~0ull;
+  page = (uint32_t)(slot / kPage);
+  return slot < (uint64_t)kv.page_count * kPage ? (int)(slot % kPage) : -1;
+}
+
+// The values' steps, minima and codes. A quotient (x - minimum) / step in f32
+// is off by at most 2^-22 of itself (difference, reciprocal and product), 4e-6
+// where it counts (up to 16): its nearest integer is certain unless it lies
+// within 1e-5 of a half h + 1/2. Then the sign of (x - minimum) - (h + 1/2) step
+// decides, which f32 holds exactly: the difference as a sum of two, the product
+// (16 bits) taken off in one fma. (16-bit values hit such a tie in one group of
+// sixty; in 64-bit arithmetic with a division the detour cost 4 of 19 us.)
+struct Grid {
+  __half step, low;
+  float s, m, r;
+};
+// (The range over 15 is rounded as a division rounds it: the quotient's
+// remainder is exact in one fma, and 1/15 has a single rounding; ranges too
+// small for that become zero steps either way.)
+static __device__ __forceinline__ Grid grid_of(float lo, float hi, bool bad) {
+  constexpr float r15 = 1.0f / 15.0f;
+  const float d = hi - lo, t = d * r15;
+  float u = fmaf(fmaf(-t, 15.0f, d), r15, t);
+  asm("" : "+v"(u));  // (rounded to 32 bits before it is to 16, not in one step)
+  Grid q;
+  q.step = bad ? __ushort_as_half(0x7E00) : __float2half_rn(u);
+  q.low = bad ? __ushort_as_half(0x7E00) : __float2half_rn(lo);
+  q.s = __half2float(q.step);
+  q.m = __half2float(q.low);
+  q.r = q.s > 0.0f ? __builtin_amdgcn_rcpf(q.s) : 0.0f;
+  return q;
+}
+// Codes of four values from bit 0 on, and the largest distance from a nearest integer.
+static __device__ __forceinline__ uint32_t codes_of(const float *x, const Grid &q, float &off) {
+  float n[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = fminf(fmaxf((x[i] - q.m) * q.r, 0.0f), 15.0f);
+    n[i] = rintf(t);
+    off = fmaxf(off, fabsf(t - n[i]));
+  }
+  return (uint32_t)fmaf(fmaf(fmaf(n[3], 16.0f, n[2]), 16.0f, n[1]), 16.0f, n[0]);
+}
+static __device__ __forceinline__ uint32_t exact_code(float x, const Grid &q) {
+  const float d = x - q.m, xx = d + q.m, rest = (x - xx) + ((xx - d) - q.m);
+  const float t = fminf(fmaxf(d * q.r, 0.0f), 15.0f), h = floorf(t);
+  if (fabsf(t - rintf(t)) <= 0.5f - 1e-5f) return (uint32_t)rintf(t);
+  const float side = fmaf(-(h + 0.5f), q.s, d) + rest;
+  return (uint32_t)h + (side > 0.0f || (side == 0.0f && ((int)h & 1)));
+}
+// Minimum and maximum, NaN where either value is, and over a quad of lanes.
+static __device__ __forceinline__ float least(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+static __device__ __forceinline__ float most(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+static __device__ __forceinline__ void over_quad(float &lo, float &hi) {
+  auto swap = [](float x, auto f) { return __int_as_float(f(__float_as_int(x))); };
+  auto one = [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, true); };
+  auto two = [](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, true); };
+  lo = least(lo, swap(lo, one));
+  hi = most(hi, swap(hi, one));
+  lo = least(lo, swap(lo, two));
+  hi = most(hi, swap(hi, two));
+}
+// Nibble i of lane 8 (l / 8) + K's word, at bit AT of w.
+template <int K, int AT>
+static __device__ __forceinline__ void nibble_of(uint32_t &w, uint32_t word, int i) {
+  w |= ((uint32_t)__builtin_amdgcn_ds_swizzle((int)word, K << 5 | 0x18) >> 4 * i & 15) << AT;
+}
+// Eight elements, as 16-byte loads where WIDE.
+template <bool WIDE, class T>
+static __device__ __forceinline__ void elements8(float (&f)[8], const T *x) {
+  if constexpr (WIDE) {
+    constexpr int N = 16 / sizeof(T);
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; i += N) *(uint4 *)(e + i) = *(const uint4 *)(x + i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = widen(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = widen(x[i]);
+  }
+}
+
+// A thread quantises eight dims 8 q .. + 7 (q = l % (HD / 8)), a quad of lanes a
+// group. K: its word of codes as it is. V: nibble j of eight threads' words, the
+// dims 16 apart that a half word holds, by broadcasts inside eights of lanes.
+// Few rows cost a launch (2.5 us of its 3.5); 16384 fp16 rows of 4 heads of 128
+// (44 MB) take 17.2 us, four fifths of it issuing vector instructions (23 a
+// value). Before: a group a thread, 64-bit divisions and byte stores 100 us; V as
+// one thread per 4 dims 16 apart (no broadcasts, but reductions over 16 lanes) 26 us.
+template <int HD, bool WIDE, class T>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4 kv, const T *k, const T *v,
                                                          size_t k_stride, size_t v_stride,
                                                          const int64_t *slots, int rows) {
-  constexpr int NG = HD / 32;
-  const int per_row = 2 * kv.heads * NG;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t r = i / per_row;
-  if (r >= rows) return;
-  const int j = (int)(i - r * per_row), g = j % NG, which = j / NG % 2, head = j / (2 * NG);
-  const int64_t slot = slots[r];
-  if (slot < 0 || slot / kPage >= (int64_t)kv.page_count) return;
-  const T *x = (which ? v + r * v_stride : k + r * k_stride) + head * HD + g * 32;
-  float lo = INFINITY, hi = -INFINITY;
-  bool bad = false;
-  for (int d = 0; d < 32; ++d) {
-    const float f = widen(x[d]);
-    bad |= !(fabsf(f) <= 32768.0f);
-    lo = fminf(lo, f);
-    hi = fmaxf(hi, f);
+  constexpr int NG = HD / 32, NH = HD / 64;
+  const StoreWave w = store_wave<HD>(kv.heads);
+  if (w.row >= rows) return;
+  const int l = threadIdx.x & 63, q = l % (HD / 8), g = q / 4, c = q % 4, r = w.row + l / (HD / 8);
+  float f[8];
+  elements8<WIDE>(f, (w.which ? v + (size_t)min(r, rows - 1) * v_stride : k + (size_t)min(r, rows - 1) * k_stride) +
+                         w.head * HD + 8 * q);
+  uint32_t page = 0;
+  const int P = place_of(kv, slots, r, rows, page);
+  float lo = least(f[0], f[1]), hi = most(f[0], f[1]);
+#pragma unroll
+  for (int i = 2; i < 8; i += 2) {
+    lo = least(least(lo, f[i]), f[i + 1]);
+    hi = most(most(hi, f[i]), f[i + 1]);
   }
-  const __half step = bad ? __ushort_as_half(0x7E00) : __float2half_rn((hi - lo) / 15.0f);
-  const __half low = bad ? __ushort_as_half(0x7E00) : __float2half_rn(lo);
-  const int P = (int)(slot % kPage);
-  uint8_t *tile = tile_of(kv, (uint32_t)(slot / kPage), head, which, 10 * HD);
-  const double s = (double)__half2float(step), m = (double)__half2float(low);
-  uint8_t code[32];
-  for (int d = 0; d < 32; ++d)
-    code[d] = s > 0.0 ? (uint8_t)fmin(fmax(rint(((double)widen(x[d]) - m) / s), 0.0), 15.0) : 0;
-  for (int d = 0; d < 32; ++d) {
-    int high;
-    const int at = code_byte<HD>(which, P, g * 32 + d, high);
-    if (!high) tile[at] = (uint8_t)(code[d] | code[d + (which ? 16 : 1)] << 4);
+  over_quad(lo, hi);
+  const Grid grid = grid_of(lo, hi, !(hi <= 32768.0f && lo >= -32768.0f));
+  float off = 0.0f;
+  uint32_t word = codes_of(f, grid, off);
+  word |= codes_of(f + 4, grid, off) << 16;
+  if (__any(off > 0.5f - 1e-5f)) {
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word |= exact_code(f[i], grid) << 4 * i;
   }
-  *(__half *)(tile + step_byte<HD>(P, g)) = step;
-  *(__half *)(tile + low_byte<HD>(which, P, g)) = low;
-}
-
-template <int HD>
-static __device__ __forceinline__ float kv4_value(const uint8_t *tile, int which, int P, int d) {
-  int high;
-  const int at = code_byte<HD>(which, P, d, high);
-  const float c = (float)(tile[at] >> (4 * high) & 15);
-  return c * __half2float(*(const __half *)(tile + step_byte<HD>(P, d / 32))) +
-         __half2float(*(const __half *)(tile + low_byte<HD>(which, P, d / 32)));
+  uint32_t half[2] = {0, 0};  // V: the half words of j = l % 8 and of j + 8
+  if (w.which) {
+    const int j = l & 7;
+    nibble_of<0, 0>(half[0], word, j);
+    nibble_of<2, 4>(half[0], word, j);
+    nibble_of<4, 8>(half[0], word, j);
+    nibble_of<6, 12>(half[0], word, j);
+    nibble_of<1, 0>(half[1], word, j);
+    nibble_of<3, 4>(half[1], word, j);
+    nibble_of<5, 8>(half[1], word, j);
+    nibble_of<7, 12>(half[1], word, j);
+  }
+  if (P < 0) return;
+  uint8_t *tile = tile_of(kv, page, w.head, w.which, 10 * HD);
+  if (w.which) {
+    uint8_t *at = tile + (((P / 4 * 16 + (l & 7)) * 2 + P / 2 % 2) * NH + q / 8) * 4 + P % 2 * 2;
+    *(uint16_t *)at = (uint16_t)half[0];
+    *(uint16_t *)(at + 8 * 2 * NH * 4) = (uint16_t)half[1];
+  } else {
+    *(uint32_t *)(tile + P * (HD / 2) + (c * NG + g) * 4) = word;
+  }
+  if (c == 0) {
+    *(__half *)(tile + step_byte<HD>(P, g)) = grid.step;
+    *(__half *)(tile + low_byte<HD>(w.which, P, g)) = grid.low;
+  }
 }
 
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 kv, const int64_t *slots, int rows,
                                                        float *k, float *v) {
-  const int width = kv.heads * HD;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t r = i / width;
-  if (r >= rows) return;
-  const int64_t slot = slots[r];
-  if (slot < 0 || slot / kPage >= (int64_t)kv.page_count) return;
-  const int d = (int)(i - r * width), head = d / HD, P = (int)(slot % kPage);
-  const uint32_t page = (uint32_t)(slot / kPage);
-  k[i] = kv4_value<HD>(tile_of(kv, page, head, 0, 10 * HD), 0, P, d % HD);
-  v[i] = kv4_value<HD>(tile_of(kv, page, head, 1, 10 * HD), 1, P, d % HD);
+  constexpr int NG = HD / 32, NH = HD / 64;
+  const StoreWave w = store_wave<HD>(kv.heads);
+  const int l = threadIdx.x & 63;
+  if (w.row >= rows) return;
+  auto half_at = [](const uint8_t *p) { return __half2float(*(const __half *)p); };
+  uint32_t page = 0;
+  if (w.which == 0) {
+    const int q = l % (HD / 8), g = q % NG, c = q / NG, r = w.row + l / (HD / 8);
+    const int P = place_of(kv, slots, r, rows, page);
+    if (P < 0) return;
+    const uint8_t *tile = tile_of(kv, page, w.head, 0, 10 * HD);
+    const uint32_t word = *(const uint32_t *)(tile + P * (HD / 2) + q * 4);
+    const float step = half_at(tile + step_byte<HD>(P, g)), low = half_at(tile + low_byte<HD>(0, P, g));
+    float4 *out = (float4 *)(k + ((size_t)r * kv.heads + w.head) * HD + 32 * g + 8 * c);
+    auto value = [&](int i) { return (float)(word >> 4 * i & 15) * step + low; };
+    out[0] = make_float4(value(0), value(1), value(2), value(3));
+    out[1] = make_float4(value(4), value(5), value(6), value(7));
+    return;
+  }
+  const int q = l % (HD / 4), h = q / 16, j = q % 16;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = w.row + u * (256 / HD) + l / (HD / 4), P = place_of(kv, slots, r, rows, page);
+    if (P < 0) continue;
+    const uint8_t *tile = tile_of(kv, page, w.head, 1, 10 * HD);
+    const uint32_t half =
+        *(const uint16_t *)(tile + (((P / 4 * 16 + j) * 2 + P / 2 % 2) * NH + h) * 4 + P % 2 * 2);
+    float *out = v + ((size_t)r * kv.heads + w.head) * HD + 64 * h + j;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      out[16 * e] = (float)(half >> 4 * e & 15) * half_at(tile + step_byte<HD>(P, 2 * h + e / 2)) +
+                    half_at(tile + low_byte<HD>(1, P, 2 * h + e / 2));
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1766,15 +1889,23 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
   return GLACIER_HIP_OK;
 }
 
+// Workgroups of an append or a read: a wave for K and one for V per head and run of rows.
+uint32_t store_grid(uint32_t rows, int heads, uint32_t hd) {
+  const uint32_t run = 512 / hd;
+  return ((rows + run - 1) / run * 2 * heads + 3) / 4;
+}
+
 template <class T>
 void append_launch(const gk::Kv4 &kv, uint32_t hd, const void *k, const void *v, uint64_t ks,
                    uint64_t vs, const int64_t *slots, uint32_t rows, hipStream_t st) {
-  const uint64_t threads = (uint64_t)rows * 2 * kv.heads * (hd / 32);
-  const uint32_t grid = (uint32_t)((threads + 255) / 256);
-  if (hd == 128)
-    gk::kv4_append_kernel<128, T><<<grid, 256, 0, st>>>(kv, (const T *)k, (const T *)v, ks, vs, slots, (int)rows);
-  else
-    gk::kv4_append_kernel<64, T><<<grid, 256, 0, st>>>(kv, (const T *)k, (const T *)v, ks, vs, slots, (int)rows);
+  const uint32_t grid = store_grid(rows, kv.heads, hd);
+  // 16-byte loads where every row's elements allow them
+  const bool wide = aligned(k, 16) && aligned(v, 16) && (ks | vs) * sizeof(T) % 16 == 0;
+  auto launch = [&](auto *kernel) {
+    kernel<<<grid, 256, 0, st>>>(kv, (const T *)k, (const T *)v, ks, vs, slots, (int)rows);
+  };
+  if (hd == 128) wide ? launch(gk::kv4_append_kernel<128, true, T>) : launch(gk::kv4_append_kernel<128, false, T>);
+  else wide ? launch(gk::kv4_append_kernel<64, true, T>) : launch(gk::kv4_append_kernel<64, false, T>);
 }
 
 }  // namespace
@@ -1857,9 +1988,7 @@ int glacier_hip_kv4_read(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t 
   DeviceScope on(ctx->device);
   GH_CHECK(ctx, on.err);
   hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
-  const uint64_t threads = (uint64_t)rows * pool->num_kv_heads * pool->head_dim;
-  if ((threads + 255) / 256 > 0x7FFFFFFFull) return GLACIER_HIP_SHAPE_MISMATCH;
-  const uint32_t grid = (uint32_t)((threads + 255) / 256);
+  const uint32_t grid = store_grid(rows, kv.heads, pool->head_dim);
   if (pool->head_dim == 128) gk::kv4_read_kernel<128><<<grid, 256, 0, st>>>(kv, slots_dev, (int)rows, k_dev, v_dev);
   else gk::kv4_read_kernel<64><<<grid, 256, 0, st>>>(kv, slots_dev, (int)rows, k_dev, v_dev);
   GH_CHECK(ctx, hipGetLastError());
