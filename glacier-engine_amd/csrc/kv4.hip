@@ -34,9 +34,13 @@ static __device__ __forceinline__ uint8_t *tile_of(const Kv4 &kv, uint32_t page,
 
 // ---------------------------------------------------------------------------
 // Planning. One workgroup, a lane a thread: two block-wide prefix sums (rows
-// and new pages), then the new table entries; the rows follow in a second
-// launch once the table is whole.
+// and new pages), then the new table entries. Few rows it writes too (a
+// row's page is an old entry or one of the free pages it hands out, so no row
+// waits for the table); many follow in a second launch. A launch is all that
+// either costs: 64 lanes take 5.1 us with 64 rows and 6.6 us with 2048 where
+// the second launch makes them 6.5 - 9.5 us; with 8192 rows it is 12.4 against 8.2.
 // ---------------------------------------------------------------------------
+constexpr uint32_t kPlanRows = 2048;  // rows that the planning workgroup writes itself
 static __device__ __forceinline__ int wave_scan(int v) {
   const int l = threadIdx.x & 63;
 #pragma unroll
@@ -50,9 +54,10 @@ static __device__ __forceinline__ int wave_scan(int v) {
 __global__ __launch_bounds__(kMaxLanes) void kv_plan_kernel(
     const int32_t *ctx, const int32_t *fresh, int lanes, int max_rows, int32_t *table,
     uint32_t max_pages, const int32_t *free_pages, uint32_t free_count, const int32_t *free_taken,
-    int32_t *row_start, int32_t *ctx_after, int32_t *result) {
+    int32_t *row_start, int32_t *ctx_after, int32_t *result, int64_t *slots, int32_t *row_lanes,
+    int32_t *row_positions) {
   __shared__ int rows_of[kMaxLanes / 64], pages_of[kMaxLanes / 64];
-  __shared__ int page_end[kMaxLanes], held_of[kMaxLanes];
+  __shared__ int page_end[kMaxLanes], held_of[kMaxLanes], rows_end[kMaxLanes], after_of[kMaxLanes];
   const int t = threadIdx.x, w = t >> 6;
   const int c = t < lanes ? ctx[t] : 0;
   int n = t < lanes ? fresh[t] : 0;
@@ -86,6 +91,8 @@ __global__ __launch_bounds__(kMaxLanes) void kv_plan_kernel(
                                                   : GLACIER_HIP_OK;
   page_end[t] = pg_end;
   held_of[t] = held;
+  rows_end[t] = row_end;
+  after_of[t] = (int)after;
   __syncthreads();  // every read of ctx and free_taken is done: they may be outputs
   const bool good = status == GLACIER_HIP_OK;
   if (t < lanes) {
@@ -99,15 +106,34 @@ __global__ __launch_bounds__(kMaxLanes) void kv_plan_kernel(
     result[2] = good ? pages : 0;
     result[3] = taken + (good ? pages : 0);
   }
-  if (!good) return;
-  for (int p = t; p < pages; p += kMaxLanes) {
-    int lo = 0, hi = kMaxLanes - 1;  // the first lane whose pages end past p
+  auto past = [](const int *ends, int i) {  // the first lane that ends past i
+    int lo = 0, hi = kMaxLanes - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (page_end[mid] > p) hi = mid;
+      if (ends[mid] > i) hi = mid;
       else lo = mid + 1;
     }
-    const int before = lo ? page_end[lo - 1] : 0;
+    return lo;
+  };
+  if (slots)
+    for (int r = t; r < max_rows; r += kMaxLanes) {
+      int64_t slot = -1;
+      int lane = -1, pos = -1;
+      if (good && r < rows) {
+        lane = past(rows_end, r);
+        pos = after_of[lane] - rows_end[lane] + r;
+        const int p = pos / kPage - held_of[lane];
+        const int page = p < 0 ? table[(size_t)lane * max_pages + pos / kPage]
+                               : free_pages[taken + (lane ? page_end[lane - 1] : 0) + p];
+        if (page >= 0) slot = (int64_t)page * kPage + pos % kPage;
+      }
+      slots[r] = slot;
+      if (row_lanes) row_lanes[r] = lane;
+      if (row_positions) row_positions[r] = pos;
+    }
+  if (!good) return;
+  for (int p = t; p < pages; p += kMaxLanes) {
+    const int lo = past(page_end, p), before = lo ? page_end[lo - 1] : 0;
     table[(size_t)lo * max_pages + held_of[lo] + (p - before)] = free_pages[taken + p];
   }
 }
@@ -1938,8 +1964,10 @@ int glacier_hip_kv_plan_rows(glacier_hip_context *ctx, const int32_t *ctx_lens_d
   hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
   gk::kv_plan_kernel<<<1, gk::kMaxLanes, 0, st>>>(
       ctx_lens_dev, new_rows_dev, (int)lanes, (int)max_rows, page_table_dev, max_pages,
-      free_pages_dev, free_count, free_taken_dev, row_start_dev, ctx_after_dev, result_dev);
+      free_pages_dev, free_count, free_taken_dev, row_start_dev, ctx_after_dev, result_dev,
+      max_rows <= gk::kPlanRows ? slots_dev : nullptr, row_lanes_dev, row_positions_dev);
   GH_CHECK(ctx, hipGetLastError());
+  if (max_rows <= gk::kPlanRows) return GLACIER_HIP_OK;
   gk::kv_plan_rows_kernel<<<(max_rows + 255) / 256, 256, 0, st>>>(
       row_start_dev, ctx_after_dev, (int)lanes, (int)max_rows, page_table_dev, max_pages, slots_dev,
       row_lanes_dev, row_positions_dev);
