@@ -42,12 +42,12 @@ static __device__ __forceinline__ uint8_t *tile_of(const Kv4 &kv, uint32_t page,
 // ---------------------------------------------------------------------------
 constexpr uint32_t kPlanRows = 2048;  // rows that the planning workgroup writes itself
 static __device__ __forceinline__ int wave_scan(int v) {
-  const int l = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o, 64);
-    if (l >= o) v += u;
-  }
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15 of rows 0, 2 onto 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31 onto the upper half
   return v;
 }
 
@@ -408,8 +408,8 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;             // waves of a workgroup
 constexpr int kRing = 2;              // pairs of pages a wave has on their way
-constexpr int kSplitPages = 2 * kWaves;   // fewest pages of a work item where a merge follows
-constexpr int kWholePages = 8 * kWaves;   // pages up to which a context stays one item
+constexpr int kUnit = 2 * kWaves * kPage;  // positions that a workgroup's waves take in one go, a pair of pages each
+constexpr int kWhole = 4;             // units up to which a context stays one item
 constexpr int kMaxSlots = 1024;       // workgroups that a batch is cut for, at most
 constexpr float kSlack = 4.0f;        // log2 units a score may pass its reference before a rescale
 constexpr float kShift = 11.0f;       // log2 of a weight at the reference
@@ -439,16 +439,6 @@ static __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
 static __device__ __forceinline__ v8h codes8(uint32_t w) {
   const uint32_t u = w >> 8;
   return as_v8h(code_pair<0, false>(w), code_pair<1, false>(w), code_pair<0, false>(u), code_pair<1, false>(u));
-}
-
-static __device__ __forceinline__ int wave_scan_dpp(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15 of rows 0, 2 onto 1, 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31 onto the upper half
-  return v;
 }
 
 // The value of lane N of each 16-lane row.
@@ -868,7 +858,7 @@ static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int leas
   const int per = (a.lanes + 63) / 64, Hkv = a.kv.heads;
   auto pages_of = [&](int i) {
     const int at = l * per + i, n = at < a.lanes ? a.ctx[at] : 0;
-    return n > 0 && n <= a.max_ctx ? (n + kPage - 1) / kPage : 0;
+    return n > 0 && n <= a.max_ctx ? (n + kUnit - 1) / kUnit : 0;
   };
   const int only = pages_of(0);
   int mine = only, live = only > 0;
@@ -877,9 +867,9 @@ static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int leas
     mine += p;
     live += p > 0;
   }
-  const int pages_in = wave_scan_dpp(mine);
+  const int pages_in = wave_scan(mine);
   const int total = __builtin_amdgcn_readlane(pages_in, 63) * Hkv;
-  const int segments = __builtin_amdgcn_readlane(wave_scan_dpp(live), 63) * Hkv;
+  const int segments = __builtin_amdgcn_readlane(wave_scan(live), 63) * Hkv;
   auto chunks_of = [&](int q) {  // of the thread's lanes
     const float r = 1.0f / (float)q;
     int n = ceil_div(only, q, r);
@@ -894,11 +884,10 @@ static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int leas
 #pragma unroll
     for (int k = 1; k < 4; ++k) {
       const int q = max(low, full - k * step);
-      if (__builtin_amdgcn_readlane(wave_scan_dpp(chunks_of(q)), 63) * Hkv <= slots) Q = q;
+      if (__builtin_amdgcn_readlane(wave_scan(chunks_of(q)), 63) * Hkv <= slots) Q = q;
     }
   }
-  Q = (Q + 1) & ~1;  // so that half of it is whole
-  const int count = chunks_of(Q) * Hkv, last = wave_scan_dpp(count);
+  const int count = chunks_of(Q) * Hkv, last = wave_scan(count);
   const int item = blockIdx.x;
   WorkItem m{-1, 0, 0, 0, 0, 0, Q};
   const uint64_t past = __ballot(last > item);
@@ -909,7 +898,7 @@ static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int leas
   const float r = 1.0f / (float)Q;
   for (int i = 0; i < per; ++i) {
     const int lane = owner * per + i, n = lane < a.lanes ? a.ctx[lane] : 0;
-    const int p = n > 0 && n <= a.max_ctx ? (n + kPage - 1) / kPage : 0;
+    const int p = n > 0 && n <= a.max_ctx ? (n + kUnit - 1) / kUnit : 0;
     const int chunks = ceil_div(p, Q, r), k = item - at;
     if (k < chunks * Hkv) {
       const int head = k / chunks;
@@ -934,21 +923,32 @@ struct DecodeLds {
 };
 
 struct MergeItem {  // of a (lane, KV head): its chunks' records
-  int start, pages, chunks, half;
+  int start, units, chunks, half;
 };
-// First page of chunk ch, and its record: the place of its first page in the
-// batch divided by half the most pages of a chunk.
-static __device__ __forceinline__ int chunk_first(int ch, int pages, int chunks) {
-  return ch * (pages / chunks) + min(ch, pages % chunks);
+// First unit of chunk ch; a chunk's record is the place of its first unit in
+// the batch divided by half the most units of a chunk.
+static __device__ __forceinline__ int chunk_first(int ch, int units, int chunks) {
+  return ch * (units / chunks) + min(ch, units % chunks);
 }
 
-// Work items: (lane, KV head, chunk of its pages), a workgroup each. Q, the
-// most pages of a chunk, comes from the batch's own lengths: the smallest of
-// a few that leaves no more items than the device holds workgroups (`slots`),
-// so that they all run at once and end together, `least` pages though. (With
-// more than slots / 2 contexts: 2 U / slots, U the batch's pages.) The chunks
-// of a context are of equal size to a page, so where there are several they
-// hold Q / 2 pages at least.
+// Work items: (lane, KV head, chunk of its units), a workgroup each; a unit is
+// what its waves take in one go. Q, the most units of a chunk, comes from the
+// batch's own lengths: the smallest of a few that leaves no more items than
+// the device holds workgroups (`slots`), so that they all run at once and end
+// together, `least` units though. (With more than slots / 2 contexts:
+// 2 U / slots, U the batch's units.) The chunks of a context are of equal size
+// to a unit, so where there are several they hold (Q + 1) / 2 units at least.
+// (Chunks equal to a page instead, whose last round leaves waves idle: 27.7
+// us instead of 23.6 for a context of 32000, 35.0 instead of 33.8 for 128 of
+// 500 to 1500; 35.3 instead of 36.3 for the 32 below.)
+//
+// 32 contexts of 1 to 8192, 28 heads of 128 over 4 (89 MB of pages): 36.3 us
+// with the merge, 31 without; the bytes take 13 at the rate of a large read.
+// What bounds it is vector instructions, 1.4 us a pair of pages and SIMD:
+// sixteen weights, their splits, and unpacking; 1.9 us find the item, 2.2 join
+// the waves. One wave a (lane, query head) took 6479 us; the same products on
+// pages loaded to registers instead of the LDS ring 48.5. Contexts of at most kWhole units are
+// not cut, so that no merge follows: its launch costs 4 to 5 us, a unit 1.5.
 template <int HD>
 __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_kernel(
     AttnArgs a, int least, int slots, MergeItem *merge, float *records) {
@@ -979,8 +979,10 @@ __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_ker
   const int ch = __builtin_amdgcn_readfirstlane(s.item.chunk), chunks = __builtin_amdgcn_readfirstlane(s.item.chunks);
   const int start = __builtin_amdgcn_readfirstlane(s.item.start), Q = __builtin_amdgcn_readfirstlane(s.item.most);
   const int lane_pages = (ctx + kPage - 1) / kPage;
-  const int first = chunk_first(ch, lane_pages, chunks), end = chunk_first(ch + 1, lane_pages, chunks);
-  if (merge && ch == 0 && t == 0) merge[lane * Hkv + h] = {start, lane_pages, chunks, Q / 2};
+  const int units = (ctx + kUnit - 1) / kUnit, first_unit = chunk_first(ch, units, chunks), half = (Q + 1) / 2;
+  const int first = first_unit * (kUnit / kPage);
+  const int end = min(chunk_first(ch + 1, units, chunks) * (kUnit / kPage), lane_pages);
+  if (merge && ch == 0 && t == 0) merge[lane * Hkv + h] = {start, units, chunks, half};
 
   Wave<HD> s_w;
 #pragma unroll
@@ -1070,7 +1072,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_ker
     s.sum[0][t] = bad ? nan : L;
   }
   __syncthreads();
-  float *rec = records + (size_t)((start + first) / (Q / 2)) * (kMaxGroup * (HD + 2));
+  float *rec = records + (size_t)((start + first_unit) / half) * (kMaxGroup * (HD + 2));
   for (int i = t; i < G * HD; i += 64 * kWaves) {
     const int g = i / HD, d = i % HD;
     const float L = s.sum[0][g];
@@ -1090,7 +1092,8 @@ __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_ker
 }
 
 // The chunks of a (lane, query head) added up, weighted by 2^(reference - the
-// largest): HD / 4 threads a record, in a fixed order.
+// largest): HD / 4 threads a record, in a fixed order. 4 to 6 us, a launch and
+// four loads that wait for each other (item, references, sums, records).
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, const MergeItem *merge,
                                                         const float *records) {
@@ -1104,7 +1107,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, const MergeI
   const MergeItem m = merge[lane * a.kv.heads + qh / G];
   if (m.chunks <= 1) return;
   auto rec = [&](int ch) {
-    return records + ((size_t)((m.start + chunk_first(ch, m.pages, m.chunks)) / m.half) * kMaxGroup + g) * (HD + 2);
+    return records + ((size_t)((m.start + chunk_first(ch, m.units, m.chunks)) / m.half) * kMaxGroup + g) * (HD + 2);
   };
   float top = -INFINITY;
   for (int ch = t; ch < m.chunks; ch += 256) {
@@ -1154,8 +1157,11 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, const MergeI
 // a workgroup (a tile). The workgroup walks the keys 32 at a time: two pages'
 // codes become values in LDS once for all columns, each as an fp16 high and
 // low part (a value keeps 22 bits; the codes' steps do not fit the operands
-// as they do with one row a head, whose weights take them), double buffered,
-// a barrier a stage:
+// as they do with one row a head, whose weights take them). The pages come
+// through an LDS ring, asked for three stages ahead by the waves in turn. V is
+// unpacked between the products of the scores, the next stage's K between
+// those of the output, so that vector instructions run beside the matrix
+// ones; a barrier follows each:
 //   scores  S^T = K . Q^T on v_mfma_f32_32x32x16_f16, high.high + high.low +
 //           low.high; lane (h, col) ends with keys 8 (i / 4) + 4 h + i % 4
 //           of its own column in register i,
@@ -1166,6 +1172,14 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, const MergeI
 //           keys are laid out in their order), so rescaling is lane-local.
 // Long contexts of few columns are cut into chunks of stages (records, merged
 // below) so that they spread over the device.
+//
+// A prompt of 2048 rows, 28 heads of 128 over 4: 131 us, 30 GFLOP, or 690
+// TFLOP/s of the three fp16 products that make one (a large library product
+// reaches 1343). A workgroup alone on a CU takes 2.05 us a stage, two 1.75 us a
+// stage between them; the matrix unit is busy 41 % of that and vector
+// instructions issue 54 %, and the two add up more than they overlap. 161 us
+// with the unpacking apart from the products. Registers (256: outputs and both
+// parts of the queries take 128) leave no third workgroup.
 typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kTile = 128;        // columns of a workgroup
 constexpr int kStage = 32;        // keys of a stage
@@ -1248,7 +1262,7 @@ static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int
         const int tiles = tiles_of(i, st, n);
         items += tiles * max(1, (st + q - 1) / q);
       }
-      return __builtin_amdgcn_readlane(wave_scan_dpp(items), 63) * Hkv;
+      return __builtin_amdgcn_readlane(wave_scan(items), 63) * Hkv;
     };
     const int room = max(slots, items_of(Q) + slots / 2);
     for (int k = 4; k <= 16; k += 2) {  // quarters of the mean
@@ -1270,10 +1284,10 @@ static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int
       cut_items += tiles * Hkv * chunks;
     }
   }
-  const int last = wave_scan_dpp(count), cut_last = wave_scan_dpp(cut), rec_last = wave_scan_dpp(cut_items);
+  const int last = wave_scan(count), cut_last = wave_scan(cut), rec_last = wave_scan(cut_items);
   // runs of more rows than there are (they overlap) have no items: the grid
   // holds those of max_rows rows
-  const bool fits = __builtin_amdgcn_readlane(wave_scan_dpp(rows), 63) <= a.max_rows;
+  const bool fits = __builtin_amdgcn_readlane(wave_scan(rows), 63) <= a.max_rows;
   const int all = fits ? __builtin_amdgcn_readlane(last, 63) : 0;
   *cut_tiles = fits ? __builtin_amdgcn_readlane(cut_last, 63) : 0;
   RowsItem m{-1, 0, 0, 0, 0, 0, 0};
@@ -1722,7 +1736,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
 // HD / 4 threads for a column (of many chunks: for one of kParts shares of
 // them, which meet in LDS), four chunks' loads on their way at a time. The
 // time is a chain of dependent loads: one thread for all chunks of a column,
-// in two passes, took 17.5 us at 42 chunks where this takes MERGE_US.
+// in two passes, took 17.5 us at 42 chunks where this takes 4.1.
 constexpr int kParts = 4, kMergeGrid = 2048;
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_rows_merge_kernel(AttnArgs a, const int *header, const RowsTile *tiles,
@@ -1873,13 +1887,14 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
   hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
   if (!row_start) {
     // a merge follows where a context may be more than one item
-    const bool split = (max_ctx + gk::kPage - 1) / gk::kPage > (uint32_t)gk::kWholePages;
-    const int least = split ? gk::kSplitPages : gk::kWholePages;
+    const uint32_t units = (max_ctx + gk::kUnit - 1) / gk::kUnit;
+    const bool split = units > (uint32_t)gk::kWhole;
+    const int least = split ? 1 : gk::kWhole;
     auto *merge = split ? (gk::MergeItem *)ws : nullptr;
     float *records = (float *)((char *)ws + merge_bytes(lanes, pool->num_kv_heads));
     const int slots = std::min(gk::kMaxSlots, ctx->props.multiProcessorCount * (pool->head_dim == 128 ? 3 : 4));
     // items at most: slots, or where there are many contexts one each and slots / 2 more
-    const uint64_t heads = (uint64_t)lanes * a.kv.heads, each = ((max_ctx + gk::kPage - 1) / gk::kPage + least - 1) / least;
+    const uint64_t heads = (uint64_t)lanes * a.kv.heads, each = (units + least - 1) / least;
     const uint64_t most = heads <= (uint64_t)slots / 2 ? slots : heads + slots / 2;
     const uint32_t grid = (uint32_t)std::max<uint64_t>(lanes, std::min(heads * each, most));
     if (pool->head_dim == 128) {
