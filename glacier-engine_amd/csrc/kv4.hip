@@ -854,7 +854,7 @@ static __device__ __forceinline__ int ceil_div(int n, int d, float rd) {
 
 // Item blockIdx.x of the list, by one wave (l its thread): a thread holds
 // a.lanes / 64 lanes.
-static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int least, int slots, int l) {
+static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int slots, int l) {
   const int per = (a.lanes + 63) / 64, Hkv = a.kv.heads;
   auto pages_of = [&](int i) {
     const int at = l * per + i, n = at < a.lanes ? a.ctx[at] : 0;
@@ -877,10 +877,10 @@ static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int leas
     return n;
   };
   const int room = max(slots - segments, slots / 2);
-  int Q = max(least, (total + room - 1) / room);
-  if (Q > least && segments < slots / 2) {
+  int Q = max(1, (total + room - 1) / room);
+  if (Q > 1 && segments < slots / 2) {
     // Q leaves slots items at most; try k / 4 of the way down to the mean
-    const int full = Q, low = max(least, (total + slots - 1) / slots), step = (Q - low + 3) / 4;
+    const int full = Q, low = max(1, (total + slots - 1) / slots), step = (Q - low + 3) / 4;
 #pragma unroll
     for (int k = 1; k < 4; ++k) {
       const int q = max(low, full - k * step);
@@ -935,8 +935,8 @@ static __device__ __forceinline__ int chunk_first(int ch, int units, int chunks)
 // what its waves take in one go. Q, the most units of a chunk, comes from the
 // batch's own lengths: the smallest of a few that leaves no more items than
 // the device holds workgroups (`slots`), so that they all run at once and end
-// together, `least` units though. (With more than slots / 2 contexts:
-// 2 U / slots, U the batch's units.) The chunks of a context are of equal size
+// together. (With more than slots / 2 contexts: 2 U / slots, U the batch's
+// units.) The chunks of a context are of equal size
 // to a unit, so where there are several they hold (Q + 1) / 2 units at least.
 // (Chunks equal to a page instead, whose last round leaves waves idle: 27.7
 // us instead of 23.6 for a context of 32000, 35.0 instead of 33.8 for 128 of
@@ -951,7 +951,7 @@ static __device__ __forceinline__ int chunk_first(int ch, int units, int chunks)
 // not cut, so that no merge follows: its launch costs 4 to 5 us, a unit 1.5.
 template <int HD>
 __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_kernel(
-    AttnArgs a, int least, int slots, MergeItem *merge, float *records) {
+    AttnArgs a, int slots, MergeItem *merge, float *records) {
   __shared__ __align__(16) DecodeLds<HD> s;
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int c = l >> 4, j = l & 15;
@@ -968,16 +968,28 @@ __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_ker
         for (int i = t; i < Hkv; i += 64 * kWaves) merge[blockIdx.x * Hkv + i].chunks = 0;
     }
   }
-  if (w == 0) {
-    const WorkItem m = find_item(a, least, slots, l);
-    if (l == 0) s.item = m;
+  int lane, h, ctx, ch = 0, chunks = 1, start = 0, Q = 1;
+  if (merge) {
+    if (w == 0) {
+      const WorkItem m = find_item(a, slots, l);
+      if (l == 0) s.item = m;
+    }
+    __syncthreads();
+    lane = __builtin_amdgcn_readfirstlane(s.item.lane);
+    if (lane < 0) return;
+    h = __builtin_amdgcn_readfirstlane(s.item.head);
+    ctx = __builtin_amdgcn_readfirstlane(s.item.ctx);
+    ch = __builtin_amdgcn_readfirstlane(s.item.chunk);
+    chunks = __builtin_amdgcn_readfirstlane(s.item.chunks);
+    start = __builtin_amdgcn_readfirstlane(s.item.start);
+    Q = __builtin_amdgcn_readfirstlane(s.item.most);
+  } else {  // contexts are items
+    lane = blockIdx.x / Hkv;
+    if (lane >= a.lanes) return;
+    h = blockIdx.x - lane * Hkv;
+    ctx = a.ctx[lane];
+    if (ctx <= 0 || ctx > a.max_ctx) return;
   }
-  __syncthreads();
-  const int lane = __builtin_amdgcn_readfirstlane(s.item.lane);
-  if (lane < 0) return;
-  const int h = __builtin_amdgcn_readfirstlane(s.item.head), ctx = __builtin_amdgcn_readfirstlane(s.item.ctx);
-  const int ch = __builtin_amdgcn_readfirstlane(s.item.chunk), chunks = __builtin_amdgcn_readfirstlane(s.item.chunks);
-  const int start = __builtin_amdgcn_readfirstlane(s.item.start), Q = __builtin_amdgcn_readfirstlane(s.item.most);
   const int lane_pages = (ctx + kPage - 1) / kPage;
   const int units = (ctx + kUnit - 1) / kUnit, first_unit = chunk_first(ch, units, chunks), half = (Q + 1) / 2;
   const int first = first_unit * (kUnit / kPage);
@@ -1889,19 +1901,18 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
     // a merge follows where a context may be more than one item
     const uint32_t units = (max_ctx + gk::kUnit - 1) / gk::kUnit;
     const bool split = units > (uint32_t)gk::kWhole;
-    const int least = split ? 1 : gk::kWhole;
     auto *merge = split ? (gk::MergeItem *)ws : nullptr;
     float *records = (float *)((char *)ws + merge_bytes(lanes, pool->num_kv_heads));
     const int slots = std::min(gk::kMaxSlots, ctx->props.multiProcessorCount * (pool->head_dim == 128 ? 3 : 4));
     // items at most: slots, or where there are many contexts one each and slots / 2 more
-    const uint64_t heads = (uint64_t)lanes * a.kv.heads, each = (units + least - 1) / least;
+    const uint64_t heads = (uint64_t)lanes * a.kv.heads, each = split ? units : 1;
     const uint64_t most = heads <= (uint64_t)slots / 2 ? slots : heads + slots / 2;
     const uint32_t grid = (uint32_t)std::max<uint64_t>(lanes, std::min(heads * each, most));
     if (pool->head_dim == 128) {
-      gk::kv4_decode_kernel<128><<<grid, 64 * gk::kWaves, 0, st>>>(a, least, slots, merge, records);
+      gk::kv4_decode_kernel<128><<<grid, 64 * gk::kWaves, 0, st>>>(a, slots, merge, records);
       if (split) gk::kv4_merge_kernel<128><<<lanes * num_heads, 256, 0, st>>>(a, merge, records);
     } else {
-      gk::kv4_decode_kernel<64><<<grid, 64 * gk::kWaves, 0, st>>>(a, least, slots, merge, records);
+      gk::kv4_decode_kernel<64><<<grid, 64 * gk::kWaves, 0, st>>>(a, slots, merge, records);
       if (split) gk::kv4_merge_kernel<64><<<lanes * num_heads, 256, 0, st>>>(a, merge, records);
     }
     GH_CHECK(ctx, hipGetLastError());
@@ -1911,7 +1922,6 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
   const int slots = std::min(gk::kRowsSlots, ctx->props.multiProcessorCount * 2);
   const int split = (max_ctx + gk::kStage - 1) / gk::kStage > (uint32_t)gk::kMinStages;
   const uint64_t tiles = (uint64_t)max_rows * (num_heads / a.kv.heads) / gk::kTile + lanes;
-  if (tiles * a.kv.heads >= (1u << 30)) return GLACIER_HIP_SHAPE_MISMATCH;
   // items at most. Chunks past the tiles' number are no more than slots less
   // the tiles or half the slots: those of cut tiles are slots at most.
   const uint32_t whole = (uint32_t)(tiles * a.kv.heads);

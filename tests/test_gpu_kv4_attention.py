@@ -219,6 +219,24 @@ def test_query_magnitudes(gh, gctx, q_gain):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("broken", [np.nan, np.inf, -np.inf])
+def test_a_broken_query_head_breaks_no_other(gh, gctx, hd, broken):
+    rng = np.random.default_rng(19)
+    ctx = [700, 90]
+    cache = Cache(rng, ctx, 2, hd)
+    q = rng.standard_normal((2, 14, hd))
+    qr = rng.standard_normal((60, 14, hd))
+    want, want_rows = decode(gh, gctx, cache, q), run_rows(gh, gctx, cache, qr, [20, 40])
+    q[0, 9, 5] = broken
+    qr[33, 3, 5] = broken
+    got, got_rows = decode(gh, gctx, cache, q), run_rows(gh, gctx, cache, qr, [20, 40])
+    assert np.isnan(got[0, 9]).all() and np.isnan(got_rows[33, 3]).all()
+    want[0, 9], got[0, 9] = 0, 0
+    want_rows[33, 3], got_rows[33, 3] = 0, 0
+    assert np.array_equal(got, want) and np.array_equal(got_rows, want_rows)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 def test_a_peak_over_a_long_flat_tail(gh, gctx, hd):
     """One key far above 5000 others whose weights, e^-14 each, still add up to
     a part in 240 of the sum: none may be rounded away. The stored keys are
