@@ -938,17 +938,16 @@ static __device__ __forceinline__ int chunk_first(int ch, int units, int chunks)
 // together. (With more than slots / 2 contexts: 2 U / slots, U the batch's
 // units.) The chunks of a context are of equal size
 // to a unit, so where there are several they hold (Q + 1) / 2 units at least.
-// (Chunks equal to a page instead, whose last round leaves waves idle: 27.7
-// us instead of 23.6 for a context of 32000, 35.0 instead of 33.8 for 128 of
-// 500 to 1500; 35.3 instead of 36.3 for the 32 below.)
+// (Chunks equal to a page instead, whose last round leaves waves idle, take a
+// context of 32000 4 us more and 128 of 500 to 1500 1.2, the 32 below 1 less.)
 //
-// 32 contexts of 1 to 8192, 28 heads of 128 over 4 (89 MB of pages): 36.3 us
+// 32 contexts of 1 to 8192, 28 heads of 128 over 4 (89 MB of pages): 34.5 us
 // with the merge, 31 without; the bytes take 13 at the rate of a large read.
 // What bounds it is vector instructions, 1.4 us a pair of pages and SIMD:
 // sixteen weights, their splits, and unpacking; 1.9 us find the item, 2.2 join
 // the waves. One wave a (lane, query head) took 6479 us; the same products on
 // pages loaded to registers instead of the LDS ring 48.5. Contexts of at most kWhole units are
-// not cut, so that no merge follows: its launch costs 4 to 5 us, a unit 1.5.
+// not cut, so that no merge follows: its launch costs 3 to 4 us, a unit 1.5.
 template <int HD>
 __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_kernel(
     AttnArgs a, int slots, MergeItem *merge, float *records) {
@@ -1188,7 +1187,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, const MergeI
 // Long contexts of few columns are cut into chunks of stages (records, merged
 // below) so that they spread over the device.
 //
-// A prompt of 2048 rows, 28 heads of 128 over 4: 131 us, 30 GFLOP, or 690
+// A prompt of 2048 rows, 28 heads of 128 over 4: 130 us, 30 GFLOP, or 690
 // TFLOP/s of the three fp16 products that make one (a large library product
 // reaches 1343). A workgroup alone on a CU takes 2.05 us a stage, two 1.75 us a
 // stage between them; the matrix unit is busy 41 % of that and vector
@@ -1198,7 +1197,10 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, const MergeI
 typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kTile = 128;        // columns of a workgroup
 constexpr int kStage = 32;        // keys of a stage
-constexpr int kMinStages = 8;     // stages of a chunk at least
+// Stages of a chunk at least, and stages up to which contexts stay whole, so
+// that no merge follows: at least 8, 4 and 2 stages a chunk take six drafting
+// lanes 19.2, 15.3 and 15.0 us, 16 rows at the end of 1000 26.6, 20.0 and 17.1.
+constexpr int kMinStages = 2, kWholeStages = 8;
 constexpr int kRowsRing = 4;      // stages whose pages are in LDS or on their way
 constexpr int kRowsSlots = 512;   // workgroups that a batch is cut for, at most
 constexpr int kRowsRecords = kRowsSlots;  // chunks of cut tiles at most
@@ -1246,7 +1248,7 @@ static __device__ __forceinline__ void run_of(const AttnArgs &a, int lane, int &
 // smallest Q of a few multiples of a slot's mean that leaves no more items
 // than slots, or than the tiles and half the slots more. (A prompt that fills
 // the device with whole tiles so stays whole: 2048 rows cut in two took 151 us
-// instead of 133, 512 rows at the end of 4096 117 instead of 138.)
+// instead of 133, 512 rows at the end of 4096 108 instead of 138.)
 // The list is dealt in runs of 256 (a CU each), every other one backwards, so
 // that CUs pair long items with short ones.
 static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int slots, bool split, int l,
@@ -1923,7 +1925,7 @@ int attention(glacier_hip_context *ctx, const glacier_hip_kv4_pool_t *pool, uint
   }
   // workgroups a CU holds
   const int slots = std::min(gk::kRowsSlots, ctx->props.multiProcessorCount * 2);
-  const int split = (max_ctx + gk::kStage - 1) / gk::kStage > (uint32_t)gk::kMinStages;
+  const int split = (max_ctx + gk::kStage - 1) / gk::kStage > (uint32_t)gk::kWholeStages;
   const uint64_t tiles = (uint64_t)max_rows * (num_heads / a.kv.heads) / gk::kTile + lanes;
   // items at most. Chunks past the tiles' number are no more than slots less
   // the tiles or half the slots: those of cut tiles are slots at most.
