@@ -513,25 +513,25 @@ static __device__ __forceinline__ void arrive() {  // all but the last N vector 
 
 template <int HD>
 static __device__ __forceinline__ void copy_pair(Slot<HD> *slot, const uint8_t *ta, const uint8_t *tb, int l) {
-  constexpr int TILE = 10 * HD;
+  constexpr int TILE = 10 * HD, kB = 64 * 16;  // bytes of a load
   const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)slot;
   // the slot's last reads are done
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   if constexpr (HD == 128) {
     const int kc = ((l & 15) * 4 + (l >> 4)) * 16;  // lane (c, j): chunk c of position j
     copy16(at, ta, kc);
-    copy16(at + 1024, tb, kc);
-    copy16(at + 2048, ta, TILE + l * 16);
-    copy16(at + 3072, tb, TILE + l * 16);
+    copy16(at + kB, tb, kc);
+    copy16(at + 2 * kB, ta, TILE + l * 16);
+    copy16(at + 3 * kB, tb, TILE + l * 16);
     const int m = l & 31;
-    copy16(at + 4096, (l < 32 ? ta : tb) + (m < 16 ? 8 * HD : TILE + 8 * HD) + (m & 15) * 16);
+    copy16(at + 4 * kB, (l < 32 ? ta : tb) + (m < 16 ? 8 * HD : TILE + 8 * HD) + (m & 15) * 16);
   } else {
     const uint8_t *t = l < 32 ? ta : tb;
     const int m = l & 31;
     copy16(at, t + m * 16);
-    copy16(at + 1024, t + TILE + m * 16);
+    copy16(at + kB, t + TILE + m * 16);
     const int x = l & 15;
-    if (l < 32) copy16(at + 2048, (l < 16 ? ta : tb) + (x < 8 ? 8 * HD : TILE + 8 * HD) + (x & 7) * 16);
+    if (l < 32) copy16(at + 2 * kB, (l < 16 ? ta : tb) + (x < 8 ? 8 * HD : TILE + 8 * HD) + (x & 7) * 16);
   }
 }
 
@@ -1283,7 +1283,7 @@ static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int
     };
     const int room = max(slots, items_of(Q) + slots / 2);
     for (int k = 4; k <= 16; k += 2) {  // quarters of the mean
-      const int q = max(kMinStages, (int)(work * (float)k / (4.0f * (float)slots)) + 1);
+      const int q = max(kMinStages, (int)fminf(work * (float)k / (4.0f * (float)slots), 1e9f) + 1);
       if (items_of(q) <= room) {
         Q = q;
         break;
