@@ -853,12 +853,12 @@ static __device__ __forceinline__ int ceil_div(int n, int d, float rd) {
 }
 
 // Item blockIdx.x of the list, by one wave (l its thread): a thread holds
-// a.lanes / 64 lanes.
-static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int slots, int l) {
+// a.lanes / 64 lanes. lens: the lanes' lengths, 0 for those that do not hold.
+static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, const int *lens, int slots, int l) {
   const int per = (a.lanes + 63) / 64, Hkv = a.kv.heads;
   auto pages_of = [&](int i) {
-    const int at = l * per + i, n = at < a.lanes ? a.ctx[at] : 0;
-    return n > 0 && n <= a.max_ctx ? (n + kUnit - 1) / kUnit : 0;
+    const int at = l * per + i;
+    return at < a.lanes ? (lens[at] + kUnit - 1) / kUnit : 0;
   };
   const int only = pages_of(0);
   int mine = only, live = only > 0;
@@ -897,8 +897,7 @@ static __device__ __forceinline__ WorkItem find_item(const AttnArgs &a, int slot
   int at = __builtin_amdgcn_readlane(last - count, owner), pb = __builtin_amdgcn_readlane(pages_in - mine, owner);
   const float r = 1.0f / (float)Q;
   for (int i = 0; i < per; ++i) {
-    const int lane = owner * per + i, n = lane < a.lanes ? a.ctx[lane] : 0;
-    const int p = n > 0 && n <= a.max_ctx ? (n + kUnit - 1) / kUnit : 0;
+    const int lane = owner * per + i, n = lane < a.lanes ? lens[lane] : 0, p = (n + kUnit - 1) / kUnit;
     const int chunks = ceil_div(p, Q, r), k = item - at;
     if (k < chunks * Hkv) {
       const int head = k / chunks;
@@ -916,6 +915,7 @@ struct DecodeLds {
   union {
     Slot<HD> ring[kWaves][kRing];
     float o[kWaves][kMaxGroup][HD];
+    int lens[kMaxLanes];
   };
   float ref[kWaves][kMaxGroup], sum[kWaves][kMaxGroup], f[kWaves][kMaxGroup];
   QueryLds<HD> query;
@@ -969,8 +969,13 @@ __global__ __launch_bounds__(64 * kWaves, HD == 128 ? 3 : 4) void kv4_decode_ker
   }
   int lane, h, ctx, ch = 0, chunks = 1, start = 0, Q = 1;
   if (merge) {
+    for (int i = t; i < a.lanes; i += 64 * kWaves) {
+      const int n = a.ctx[i];
+      s.lens[i] = n > 0 && n <= a.max_ctx ? n : 0;
+    }
+    __syncthreads();
     if (w == 0) {
-      const WorkItem m = find_item(a, slots, l);
+      const WorkItem m = find_item(a, s.lens, slots, l);
       if (l == 0) s.item = m;
     }
     __syncthreads();
@@ -1251,14 +1256,15 @@ static __device__ __forceinline__ void run_of(const AttnArgs &a, int lane, int &
 // instead of 133, 512 rows at the end of 4096 108 instead of 138.)
 // The list is dealt in runs of 256 (a CU each), every other one backwards, so
 // that CUs pair long items with short ones.
-static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int slots, bool split, int l,
-                                                          int *cut_tiles) {
+// runs: the lanes' rows and stages.
+static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, const int2 *runs, int slots, bool split,
+                                                          int l, int *cut_tiles) {
   const int per = (a.lanes + 63) / 64, Hkv = a.kv.heads, G = a.num_heads / Hkv;
   auto tiles_of = [&](int i, int &stages, int &n) {
-    int first;
-    run_of(a, l * per + i, first, n);
-    const int ctx = n > 0 ? a.ctx[l * per + i] : 0;
-    stages = ctx >= n && ctx <= a.max_ctx ? (ctx + kStage - 1) / kStage : 0;
+    const int at = l * per + i;
+    const int2 r = at < a.lanes ? runs[at] : int2{0, 0};
+    n = r.x;
+    stages = r.y;
     return (n * G + kTile - 1) / kTile;
   };
   int n0, st0;
@@ -1317,10 +1323,8 @@ static __device__ __forceinline__ RowsItem find_rows_item(const AttnArgs &a, int
   int rec_at = __builtin_amdgcn_readlane(rec_last - cut_items, owner);
   for (int i = 0; i < per; ++i) {
     const int lane = owner * per + i;
-    int first, n;
-    run_of(a, lane, first, n);
-    const int ctx = n > 0 ? a.ctx[lane] : 0;
-    const int st = ctx >= n && ctx <= a.max_ctx ? (ctx + kStage - 1) / kStage : 0;
+    const int2 run_here = lane < a.lanes ? runs[lane] : int2{0, 0};
+    const int n = run_here.x, st = run_here.y;
     const int tiles = (n * G + kTile - 1) / kTile, chunks = max(1, (st + Q - 1) / Q), k = item - at;
     const int here = tiles * Hkv * chunks;
     if (k < here) {
@@ -1487,9 +1491,17 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
   const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int Hkv = a.kv.heads, G = a.num_heads / Hkv;
   const float nan = __uint_as_float(0x7FC00000u);
+  static_assert(sizeof(s.k) >= kMaxLanes * sizeof(int2), "the lanes' runs lie where the keys come later");
+  for (int i = t; i < a.lanes; i += 256) {
+    int first, n;
+    run_of(a, i, first, n);
+    const int ctx = a.ctx[i];
+    ((int2 *)s.k)[i] = {n, n > 0 && ctx >= n && ctx <= a.max_ctx ? (ctx + kStage - 1) / kStage : 0};
+  }
+  __syncthreads();
   if (w == 0) {
     int cut;
-    const RowsItem m = find_rows_item(a, slots, split, l, &cut);
+    const RowsItem m = find_rows_item(a, (const int2 *)s.k, slots, split, l, &cut);
     if (l == 0) {
       s.item[0] = m.lane;
       s.item[1] = m.head;
