@@ -1192,7 +1192,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttnArgs a, const MergeI
 // Long contexts of few columns are cut into chunks of stages (records, merged
 // below) so that they spread over the device.
 //
-// A prompt of 2048 rows, 28 heads of 128 over 4: 130 us, 30 GFLOP, or 690
+// A prompt of 2048 rows, 28 heads of 128 over 4: 131 us, 30 GFLOP, or 690
 // TFLOP/s of the three fp16 products that make one (a large library product
 // reaches 1343). A workgroup alone on a CU takes 2.05 us a stage, two 1.75 us a
 // stage between them; the matrix unit is busy 41 % of that and vector
@@ -1637,13 +1637,15 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
       };
       read_k(0);
       read_k(1);
+      // the matrix products' wave first: the other workgroup's fills their gaps
+      // (eight mixed lanes 61.7 -> 59.5 us)
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < S; i += 2) {
         if (i + 2 < S) {
           read_k(i + 2);
           read_k(i + 3);
         }
-        __builtin_amdgcn_sched_barrier(0);  // (the next operands before this step's products)
         sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[i & 3], ql[i], sc, 0, 0, 0);
         sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[i + 1 & 3], ql[i + 1], sd, 0, 0, 0);
         value_part(s, rv, i / 2, page, part, l);
@@ -1653,6 +1655,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
         sd = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[i + 1 & 3], qh[i + 1], sd, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
       sc += sd;
       if (key0 + kStage > wave_first) {
         asm volatile("");
@@ -1700,6 +1703,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
       };
       read_v(0);
       read_v(1);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < 2 * NG; i += 2) {
         const int x = i / NG, g = i % NG;
@@ -1707,7 +1711,6 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
           read_v(i + 2);
           read_v(i + 3);
         }
-        __builtin_amdgcn_sched_barrier(0);
         const v8h bh = as_v8h(ph[4 * x], ph[4 * x + 1], ph[4 * x + 2], ph[4 * x + 3]);
         const v8h bl = as_v8h(pl[4 * x], pl[4 * x + 1], pl[4 * x + 2], pl[4 * x + 3]);
         o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[i & 3], bl, o[g], 0, 0, 0);
@@ -1720,6 +1723,7 @@ __global__ __launch_bounds__(256, 2) void kv4_rows_kernel(AttnArgs a, int slots,
         o[g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh[i + 1 & 3], bh, o[g + 1], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
       if (__builtin_amdgcn_readfirstlane(s.odd[st & 1][NG])) {
         const int k = min(kStage, seen - key0);
         const uint32_t shown = k <= 0 ? 0u : k >= 32 ? 0xFFFFFFFFu : (1u << k) - 1;
