@@ -404,7 +404,6 @@ struct AttnArgs {
 // Decode attention
 // ---------------------------------------------------------------------------
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;             // waves of a workgroup
 constexpr int kRing = 2;              // pairs of pages a wave has on their way
